@@ -17,7 +17,9 @@ BUILD_DIR = os.path.join(HERE, "_build")
 SOURCES = [os.path.join(HERE, "hip", f)
            for f in ("bindings.cpp", "norms.hip", "gemm_mfma.hip",
                      "optim.hip", "attention.hip", "bn.hip", "ce.hip",
-                     "elementwise.hip", "embedding.hip")]
+                     "elementwise.hip", "embedding.hip",
+                     "attention_packed.hip", "rope_axes.hip",
+                     "block_norm.hip", "clip.hip")]
 EXT_NAME = "_hip_ops"
 
 
@@ -32,7 +34,11 @@ def build_ext(verbose: bool = False):
         sources=sources,
         build_directory=BUILD_DIR,
         extra_cflags=["-O3"],
-        extra_cuda_cflags=["-O3", "-std=c++17"],
+        # without packed fp32 (v_pk_*_f32): some of its forms have given
+        # wrong results on this card
+        extra_cuda_cflags=["-O3", "-std=c++17", "-Xclang",
+                           "-target-feature", "-Xclang",
+                           "-packed-fp32-ops"],
         verbose=verbose,
     )
     return mod
