@@ -12,6 +12,7 @@ composite (tests).
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 
@@ -109,3 +110,134 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         k = k.repeat_interleave(rep, dim=1)
         v = v.repeat_interleave(rep, dim=1)
     return _ref_attention(q, k, v, causal)
+
+
+class _FlashAttnPackedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, lengths, causal, window, scale):
+        ext = get_ext(required=True)
+        o, lse = ext.attn_packed_fwd(q, k, v, cu_seqlens, lengths, causal,
+                                     window, scale)
+        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens, lengths)
+        ctx.causal, ctx.window, ctx.scale = causal, window, scale
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        # probabilities are computed again from lse, nothing T x T is kept
+        ext = get_ext(required=True)
+        q, k, v, o, lse, cu_seqlens, lengths = ctx.saved_tensors
+        dq, dk, dv = ext.attn_packed_bwd(
+            q, k, v, o, _aligned_rows(do), lse, cu_seqlens, lengths,
+            ctx.causal, ctx.window, ctx.scale)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it where the kernels' 16-byte reads cannot follow
+    its strides.  (stride 0 is fine: every row is the same one.)"""
+    if x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 \
+            and x.data_ptr() % 16 == 0:
+        return x
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _ref_attention_packed(q, k, v, cu_seqlens, lengths, causal, window,
+                          scale):
+    # fp32 composite; used on CPU
+    T, H, D = q.shape
+    rep = H // k.shape[1]
+    o = torch.zeros(T, H, D, dtype=torch.float32, device=q.device)
+    cu = [min(max(int(c), 0), T) for c in cu_seqlens.tolist()]
+    lens = (lengths.tolist() if lengths is not None
+            else [T] * (len(cu) - 1))
+    parts, at = [], 0
+    for b, e, n in zip(cu[:-1], cu[1:], lens):
+        n = min(max(int(n), 0), max(e - b, 0))
+        if n == 0:
+            continue
+        qs, ks, vs = (x[b:b + n].float().transpose(0, 1) for x in (q, k, v))
+        ks, vs = (x.repeat_interleave(rep, dim=0) for x in (ks, vs))
+        s = torch.matmul(qs, ks.transpose(-1, -2)) * scale
+        far = torch.arange(n)[:, None] - torch.arange(n)
+        if causal:
+            s = s.masked_fill(far < 0, float("-inf"))
+        if window:
+            s = s.masked_fill(far >= window, float("-inf"))
+        out = torch.matmul(torch.softmax(s, dim=-1), vs).transpose(0, 1)
+        parts += [o[at:b], out]
+        at = b + n
+    return torch.cat(parts + [o[at:]]).to(q.dtype)
+
+
+def flash_attention_packed(q: torch.Tensor, k: torch.Tensor,
+                           v: torch.Tensor, cu_seqlens: torch.Tensor,
+                           lengths: Optional[torch.Tensor] = None,
+                           causal: bool = False,
+                           window: Optional[int] = None,
+                           scale: Optional[float] = None) -> torch.Tensor:
+    """Self-attention within each of several packed sequences.
+
+    ``q`` [T, H, D], ``k``, ``v`` [T, HK, D] (HK divides H), bf16 or
+    fp16, D a multiple of 8 up to 128; slices of a fused projection are
+    read in place.  ``cu_seqlens`` int32 [sequences + 1], on q's device:
+    sequence i is rows ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``; it
+    begins with 0 and does not fall, and rows behind its last value
+    belong to no sequence.  ``lengths`` int32 [sequences]: only the
+    first ``lengths[i]`` rows of sequence i are tokens, the rest is
+    padding (a padded batch [B, S] is ``cu_seqlens = [0, S, 2S, ...]``).
+
+    ``causal``: a row sees its own and earlier rows; ``window`` (causal
+    only): of those the last ``window``, its own among them.  ``scale``
+    defaults to 1/sqrt(D).
+
+    Returns o [T, H, D], contiguous.  Rows that are no tokens get zeros,
+    in o and in the gradients, whatever they hold.  An infinity or NaN
+    stays in its own sequence.  Where cu_seqlens falls or leaves [0, T]
+    the result is undefined, but nothing outside the tensors is
+    touched.  Nothing here waits for the GPU; a call can be captured."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape \
+            or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"flash_attention_packed: q [T, H, D], k and v "
+                         f"[T, HK, D] wanted, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    T, H, D = q.shape
+    if k.shape[1] < 1 or H < 1 or H % k.shape[1]:
+        raise ValueError(f"flash_attention_packed: {k.shape[1]} kv heads do "
+                         f"not divide {H} heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"flash_attention_packed: D must be a multiple of "
+                         f"8, at most 128, got {D}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 \
+            or cu_seqlens.dtype != torch.int32:
+        raise ValueError("flash_attention_packed: cu_seqlens must be int32 "
+                         "[sequences + 1]")
+    if lengths is not None and (lengths.dtype != torch.int32 or
+                                lengths.shape != (cu_seqlens.numel() - 1,)):
+        raise ValueError("flash_attention_packed: lengths must be int32 "
+                         "[sequences]")
+    for t in (k, v, cu_seqlens, lengths):
+        if t is not None and t.device != q.device:
+            raise ValueError("flash_attention_packed: all tensors must be "
+                             "on one device")
+    if window is not None and (not causal or window < 1):
+        raise ValueError("flash_attention_packed: window must be at least "
+                         "1, and needs causal")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"flash_attention_packed: scale is {scale}")
+    if q.is_cuda:
+        if q.dtype not in (torch.bfloat16, torch.float16) \
+                or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise ValueError(f"flash_attention_packed: q, k and v must all "
+                             f"be bf16 or fp16, got {q.dtype}, {k.dtype}, "
+                             f"{v.dtype}")
+        return _FlashAttnPackedFn.apply(
+            _aligned_rows(q), _aligned_rows(k), _aligned_rows(v),
+            cu_seqlens.contiguous(),
+            None if lengths is None else lengths.contiguous(), causal,
+            window or 0, scale)
+    return _ref_attention_packed(q, k, v, cu_seqlens, lengths, causal,
+                                 window, scale)

@@ -1,6 +1,8 @@
 """Fused RoPE and SwiGLU-gate wrappers (ops/hip/elementwise.hip)."""
 from __future__ import annotations
 
+from typing import Sequence
+
 import torch
 
 from ._ext import get_ext
@@ -31,6 +33,99 @@ def fused_rope(x: torch.Tensor, cosb: torch.Tensor,
     s = sinb[:S].to(x.dtype)[None, None]
     x1, x2 = x.chunk(2, dim=-1)
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
+
+
+class _RopeAxesFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, cosb, sinb, sections):
+        ext = get_ext(required=True)
+        ctx.save_for_backward(positions, cosb, sinb)
+        ctx.sections = sections
+        return tuple(ext.rope_axes(q, k, positions, cosb, sinb, sections,
+                                   False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        ext = get_ext(required=True)
+        positions, cosb, sinb = ctx.saved_tensors
+        dq, dk = ext.rope_axes(_dense_rows(dq), _dense_rows(dk), positions,
+                               cosb, sinb, ctx.sections, True)
+        return dq, dk, None, None, None, None
+
+
+def _dense_rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
+                    positions: torch.Tensor, cosb: torch.Tensor,
+                    sinb: torch.Tensor, sections: Sequence[int]):
+    """Rotate-half RoPE by token positions on one or several axes.
+
+    ``q`` [T, H, D], ``k`` [T, HK, D]: packed tokens (slices of a fused
+    projection are read in place).  ``positions`` [axes, T], int32 or
+    int64: each token's position on each axis, e.g. time, height and
+    width; the positions of packed sequences restart at will.  ``cosb``,
+    ``sinb`` [P, R/2] fp32: row p holds the angles of position p.
+    ``sections``: how many of the R/2 frequencies, in order, go by each
+    axis (``[R/2]`` for one axis).  Values from R on (R <= D) pass
+    through.  1 to 4 axes; q and k both bf16, fp16 or fp32.
+
+    Returns new contiguous ``(q, k)``.  A position outside of the tables
+    makes that token's values on that axis NaN."""
+    sections = [int(n) for n in sections]
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] \
+            or q.shape[2] != k.shape[2]:
+        raise ValueError(f"fused_rope_axes: q [T, H, D] and k [T, HK, D] "
+                         f"wanted, got {tuple(q.shape)}, {tuple(k.shape)}")
+    if q.dtype != k.dtype or q.dtype not in (torch.bfloat16, torch.float16,
+                                             torch.float32):
+        raise ValueError(f"fused_rope_axes: q and k must both be bf16, fp16 "
+                         f"or fp32, got {q.dtype}, {k.dtype}")
+    if cosb.dim() != 2 or cosb.shape != sinb.shape \
+            or cosb.dtype != torch.float32 or sinb.dtype != torch.float32:
+        raise ValueError("fused_rope_axes: cosb and sinb must be fp32 "
+                         "[places, R/2]")
+    half = cosb.shape[1]
+    if not 1 <= len(sections) <= 4 or min(sections) < 1 \
+            or sum(sections) != half or 2 * half > q.shape[2]:
+        raise ValueError(f"fused_rope_axes: sections {sections} must be 1 to "
+                         f"4 positive counts that add up to {half}, at most "
+                         f"half of D = {q.shape[2]}")
+    if positions.shape != (len(sections), q.shape[0]) \
+            or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"fused_rope_axes: positions must be int32 or int64 "
+                         f"[{len(sections)}, {q.shape[0]}], got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    for t in (k, positions, cosb, sinb):
+        if t.device != q.device:
+            raise ValueError("fused_rope_axes: all tensors must be on one "
+                             "device")
+    if q.is_cuda:
+        return _RopeAxesFn.apply(_dense_rows(q), _dense_rows(k),
+                                 positions.contiguous(), cosb.contiguous(),
+                                 sinb.contiguous(), sections)
+    axis = torch.repeat_interleave(torch.arange(len(sections)),
+                                   torch.tensor(sections))
+    at = positions[axis].t().long()                        # [T, R/2]
+    ok = (at >= 0) & (at < cosb.shape[0])
+    nan = torch.full((), float("nan"))
+    if cosb.shape[0]:
+        at = at.clamp(0, cosb.shape[0] - 1)
+        place = torch.arange(half)
+        c, s = (torch.where(ok, b[at, place], nan)[:, None]
+                for b in (cosb, sinb))
+    else:
+        c = s = nan.expand(q.shape[0], 1, half)
+
+    def turn(x):
+        a, b = x[..., :half].float(), x[..., half:2 * half].float()
+        return torch.cat([(a * c - b * s).to(x.dtype),
+                          (b * c + a * s).to(x.dtype),
+                          x[..., 2 * half:]], dim=-1)
+
+    return turn(q), turn(k)
 
 
 class _SiluMulFn(torch.autograd.Function):

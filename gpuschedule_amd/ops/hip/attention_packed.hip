@@ -1,0 +1,688 @@
+// Attention over packed sequences for gfx950: forward and backward.
+//
+// q [T, H, D], k and v [T, HK, D] hold the sequences one behind the other;
+// sequence i is rows cu[i]..cu[i+1], of which the first lengths[i] are
+// tokens and the rest padding.  Per head, with the keys j that row i sees:
+//   s = scale q.k,  p = exp(s - lse),  lse = log sum exp(s),  o = p v
+//   dV = p^T dO,  dP = dO v^T,  dS = scale p (dP - D),  D = dO.o
+//   dQ = dS k,  dK = dS^T q          (backward computes p again from lse)
+//
+// Matrix work is v_mfma_f32_32x32x16.  Its accumulator holds, in lane l,
+// column l % 32 and rows 8 (i / 4) + 4 (l / 32) + i % 4: a product whose
+// operands are swapped so that the softmax's row is the COLUMN leaves every
+// lane with 16 values of one row.  Its maximum and sum need one exchange
+// between lanes l and l ^ 32, and the 16 values, rounded, ARE the second
+// product's B operand if that product takes its reduction in the order in
+// which they stand.  Its A operand comes out of LDS through transposing
+// reads of 4 neighbouring rows, which give exactly that order.  So
+// probabilities never pass through LDS, and no transposed copy is made.
+//
+// Sequences are found on the GPU: a call waits for nothing and can be
+// captured.  A tile of R rows lies in one sequence; sequence i owns the
+// slots from cu[i] / R + i on, which is at least as many as it has tiles,
+// so that a slot's sequence is a binary search over cu and the number of
+// slots, T / R + sequences + 1, is known on the host.  Rows behind the last
+// sequence count as one more, without tokens.  Rows without tokens get
+// zeros.
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <cmath>
+#include "common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) unsigned uint4v;
+
+struct BF {
+  static __device__ __forceinline__ float16v mfma(short8 a, short8 b,
+                                                  float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+        0);
+  }
+  static __device__ __forceinline__ short8 pack(const float* v) {
+    bf16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (__bf16)v[j];
+    return __builtin_bit_cast(short8, r);
+  }
+  static __device__ __forceinline__ short one(float v) {
+    return __builtin_bit_cast(short, (__bf16)v);
+  }
+  static __device__ __forceinline__ float up(short v) { return bf16_to_f32(v); }
+};
+
+struct FH {
+  static __device__ __forceinline__ float16v mfma(short8 a, short8 b,
+                                                  float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+        0);
+  }
+  static __device__ __forceinline__ short8 pack(const float* v) {
+    f16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (_Float16)v[j];
+    return __builtin_bit_cast(short8, r);
+  }
+  static __device__ __forceinline__ short one(float v) {
+    return __builtin_bit_cast(short, (_Float16)v);
+  }
+  static __device__ __forceinline__ float up(short v) {
+    return (float)__builtin_bit_cast(_Float16, v);
+  }
+};
+
+constexpr int NW = 4, NTH = NW * 64;
+constexpr int TILE = 64;           // rows of a staged tile
+constexpr int OWN = 32 * NW;       // rows that a block owns: 32 a wave
+
+struct Args {
+  const short *q, *k, *v, *o, *dout;
+  short *out, *dq, *dk, *dv;
+  float *lse, *drow;               // [H, T]; lse in units of log 2
+  const int *cu, *lengths;         // lengths may be null
+  long q_t, q_h, k_t, k_h, v_t, v_h, d_t, d_h;  // strides; d: dout
+  int T, B, H, HK, D, units, window;            // window 0: none
+  float scale;
+};
+
+__device__ const uint4v kZeros = {0, 0, 0, 0};
+
+// ---- which rows --------------------------------------------------------
+
+struct Seq {
+  int begin, rows, len;            // first row, all rows, tokens
+};
+
+__device__ __forceinline__ int bound_of(const Args& a, int i) {
+  return i > a.B ? a.T : min(max(a.cu[i], 0), a.T);
+}
+
+// The sequence and first row (in it) of a slot; false: the slot is not used.
+template <int R>
+__device__ __forceinline__ bool tile_of(const Args& a, int slot, Seq& s,
+                                        int& row0) {
+  int lo = 0, hi = a.B;            // the last i whose slots begin at or before
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (bound_of(a, mid) / R + mid <= slot) lo = mid; else hi = mid - 1;
+  }
+  s.begin = bound_of(a, lo);
+  s.rows = max(bound_of(a, lo + 1) - s.begin, 0);
+  s.len = lo == a.B ? 0 : s.rows;
+  if (a.lengths && lo < a.B) s.len = min(max(a.lengths[lo], 0), s.rows);
+  row0 = (slot - (s.begin / R + lo)) * R;
+  return row0 >= 0 && row0 < s.rows;
+}
+
+// A unit is one kv head's share of one slot; its `rep` query heads are
+// neighbours in time on one XCD (blocks go to the 8 XCDs in turn), so that
+// they find its keys in that XCD's L2.  kv heads change fastest, so that
+// every XCD gets tiles of all places; late slots, the long ones under a
+// causal mask, go first.
+__device__ __forceinline__ bool unit_of(const Args& a, int rep, int& kvh,
+                                        int& slot, int& sub) {
+  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+  const int unit = j / rep * 8 + xcd;
+  sub = j % rep;
+  kvh = unit % a.HK;
+  slot = a.units / a.HK - 1 - unit / a.HK;
+  return unit < a.units;
+}
+
+// ---- LDS tiles ---------------------------------------------------------
+// A tile is [TILE][DP] with its 16-byte chunks swizzled: chunk c of row r
+// stands at c ^ mix(r).  Two kinds of reads have to miss each other's banks
+// (64 of 4 bytes): 16 rows at one chunk, and 4 neighbouring rows at 64
+// neighbouring bytes.
+
+template <int DP> __device__ __forceinline__ int mix(int r) {
+  if constexpr (DP == 128) return (r & 3) << 2 | (r >> 2 & 3);
+  return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
+}
+
+// Rows row0.. of p (row stride `ld`) to LDS without passing registers.
+// Rows from `rows` on and values from D on are zeros: those lanes read
+// zeros instead, so nothing of another sequence ever enters a product.
+template <int DP>
+__device__ __forceinline__ void stage(const short* p, long ld, int row0,
+                                      int rows, int D, char* tile) {
+  constexpr int NCH = DP / 8;
+#pragma unroll
+  for (int it = 0; it < TILE * NCH / NTH; ++it) {
+    const int at = it * NTH + threadIdx.x;
+    const int r = at / NCH, c = (at % NCH) ^ mix<DP>(r);
+    const bool ok = row0 + r < rows && c * 8 < D;
+    const short* g = p + (long)(row0 + r) * ld + c * 8;
+    const void* src = ok ? (const void*)g : (const void*)&kZeros;
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) unsigned*)src,
+        (__attribute__((address_space(3))) unsigned*)
+            (tile + (it * NTH + (threadIdx.x & ~63)) * 16),
+        16, 0, 0);
+  }
+}
+
+// A operand from rows: row r0 + l % 32, values 16 kk + 8 (l / 32) + 0..7.
+template <int DP>
+__device__ __forceinline__ short8 rows_of(const char* tile, int r0, int kk,
+                                          int lane) {
+  const int r = r0 + (lane & 31), c = 2 * kk + (lane >> 5);
+  return *reinterpret_cast<const short8*>(tile + r * DP * 2 +
+                                          ((c ^ mix<DP>(r)) << 4));
+}
+
+// A operand from columns: value 32 f + l % 32 of 8 rows, in the order of an
+// accumulator: rows r0 + 4 (l / 32) + 0..3 and r0 + 8 + 4 (l / 32) + 0..3.
+// In a transposing read the 16 lanes of a group name 4 rows of 16 values,
+// 4 values each, and lane j of the group gets value j of the 4 rows.
+template <int DP>
+__device__ __forceinline__ short8 cols_of(const char* tile, int r0, int f,
+                                          int lane) {
+  short4v part[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int j = lane & 15;
+    const int r = r0 + 8 * b + 4 * (lane >> 5) + (j >> 2);
+    const int c = 4 * f + (lane >> 4 & 1) * 2 + (j >> 1 & 1);
+    const char* at = tile + r * DP * 2 + ((c ^ mix<DP>(r)) << 4) + (j & 1) * 8;
+    part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) short4v*)at);
+  }
+  return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// B operand straight from global memory: row of this lane, DP / 16 steps.
+template <int DP>
+__device__ __forceinline__ void own_rows(const short* p, bool ok, int D,
+                                         int lane, short8 (&v)[DP / 16]) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int d = 16 * kk + 8 * (lane >> 5);
+    v[kk] = ok && d < D ? *reinterpret_cast<const short8*>(p + d)
+                        : short8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+}
+
+// The accumulator of a [DP][32 rows] product: lane's row gets its values.
+template <class E, int DP>
+__device__ __forceinline__ void put_rows(short* p, bool live, int D, int lane,
+                                         float by, const float16v (&acc)[DP / 32]) {
+#pragma unroll
+  for (int f = 0; f < DP / 32; ++f)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * f + 8 * g + 4 * (lane >> 5);
+      short4v w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = live ? E::one(acc[f][4 * g + j] * by) : (short)0;
+      if (d < D) *reinterpret_cast<short4v*>(p + d) = w;
+    }
+}
+
+// The other half's value (lane l ^ 32).
+__device__ __forceinline__ float other_half(float v) {
+  return __shfl_xor(v, 32, WAVE);
+}
+
+constexpr float kNone = -INFINITY;
+
+// ---- forward -----------------------------------------------------------
+
+template <class E, int DP, bool CAUSAL>
+__global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rep = a.H / a.HK;
+  int kvh, slot, sub, row0;
+  Seq s;
+  if (!unit_of(a, rep, kvh, slot, sub)) return;
+  if (!tile_of<OWN>(a, slot, s, row0)) return;
+  const int head = kvh * rep + sub;
+  const int row = row0 + wave * 32 + (lane & 31);
+  const bool live = row < s.len;
+  const long at = s.begin + row;
+
+  float m = kNone, l = 0.f;
+  float16v o[DP / 32];
+#pragma unroll
+  for (int f = 0; f < DP / 32; ++f) o[f] = (float16v)(0.f);
+
+  if (row0 < s.len) {
+    short8 q[DP / 16];
+    own_rows<DP>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
+    const short* kp = a.k + (long)s.begin * a.k_t + kvh * a.k_h;
+    const short* vp = a.v + (long)s.begin * a.v_t + kvh * a.v_h;
+    const int end = CAUSAL ? min(s.len, row0 + OWN) : s.len;
+    int t0 = 0;
+    if (a.window) t0 = max(row0 - a.window + 1, 0) / TILE;
+    const int t1 = (end + TILE - 1) / TILE;
+    const int first = row0 + wave * 32, last = first + 31;
+    const float sl2 = a.scale * 1.44269504088896340736f;
+    stage<DP>(kp, a.k_t, t0 * TILE, s.len, a.D, lds[0]);
+    stage<DP>(vp, a.v_t, t0 * TILE, s.len, a.D, lds[1]);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int kv0 = t * TILE;
+      char* kt = lds[(t - t0) & 1 ? 2 : 0];
+      char* vt = lds[(t - t0) & 1 ? 3 : 1];
+      if (t + 1 < t1) {
+        stage<DP>(kp, a.k_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 0 : 2]);
+        stage<DP>(vp, a.v_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 1 : 3]);
+      }
+      if ((!CAUSAL || kv0 <= last) && first < s.len &&
+          (!a.window || kv0 + TILE > first - a.window + 1)) {
+        float16v sc[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          sc[kb] = (float16v)(0.f);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            sc[kb] = E::mfma(rows_of<DP>(kt, 32 * kb, kk, lane), q[kk], sc[kb]);
+        }
+        const bool edge = kv0 + TILE > s.len ||
+                          (CAUSAL && kv0 + TILE - 1 > first) ||
+                          (a.window && kv0 <= last - a.window);
+        if (edge) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) +
+                              i % 4;
+              bool seen = key < s.len;
+              if (CAUSAL) seen &= key <= row;
+              if (a.window) seen &= key > row - a.window;
+              if (!seen) sc[kb][i] = kNone;
+            }
+        }
+        float top = kNone;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
+        top = fmaxf(top, other_half(top)) * sl2;
+        const float mn = fmaxf(m, top);
+        const float ref = mn == kNone ? 0.f : mn;
+        const float alpha = exp2f(m - ref);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int f = 0; f < DP / 32; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[f][i] *= alpha;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            p[j] = exp2f(sc[ks / 2][8 * (ks & 1) + j] * sl2 - ref);
+            l += p[j];
+          }
+          // probabilities are rounded to the type of v, which the matrix
+          // product needs; their sum is taken before
+          const short8 pb = E::pack(p);
+#pragma unroll
+          for (int f = 0; f < DP / 32; ++f)
+            o[f] = E::mfma(cols_of<DP>(vt, 16 * ks, f, lane), pb, o[f]);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  l += other_half(l);
+  if (row < s.rows) {
+    put_rows<E, DP>(a.out + (at * a.H + head) * a.D, live, a.D, lane, 1.f / l,
+                    o);
+    // a row without keys: exp(s - inf) is 0 in backward
+    if (lane < 32)
+      a.lse[(long)head * a.T + at] = live ? m + log2f(l) : INFINITY;
+  }
+}
+
+// ---- backward: dQ, and D for the other kernel --------------------------
+
+template <class E, int DP, bool CAUSAL>
+__global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rep = a.H / a.HK;
+  int kvh, slot, sub, row0;
+  Seq s;
+  if (!unit_of(a, rep, kvh, slot, sub)) return;
+  if (!tile_of<OWN>(a, slot, s, row0)) return;
+  const int head = kvh * rep + sub;
+  const int row = row0 + wave * 32 + (lane & 31);
+  const bool live = row < s.len;
+  const long at = s.begin + row;
+
+  float16v dq[DP / 32];
+#pragma unroll
+  for (int f = 0; f < DP / 32; ++f) dq[f] = (float16v)(0.f);
+
+  if (row0 < s.len) {
+    short8 q[DP / 16], dO[DP / 16];
+    own_rows<DP>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
+    own_rows<DP>(a.dout + at * a.d_t + head * a.d_h, live, a.D, lane, dO);
+    float dr = 0.f;
+    {
+      short8 ov[DP / 16];
+      own_rows<DP>(a.o + (at * a.H + head) * a.D, live, a.D, lane, ov);
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          dr += E::up(ov[kk][j]) * E::up(dO[kk][j]);
+      dr = (dr + other_half(dr)) * a.scale;
+    }
+    const float lse = live ? a.lse[(long)head * a.T + at] : INFINITY;
+    if (live && lane < 32) a.drow[(long)head * a.T + at] = dr;
+    const short* kp = a.k + (long)s.begin * a.k_t + kvh * a.k_h;
+    const short* vp = a.v + (long)s.begin * a.v_t + kvh * a.v_h;
+    const int end = CAUSAL ? min(s.len, row0 + OWN) : s.len;
+    int t0 = 0;
+    if (a.window) t0 = max(row0 - a.window + 1, 0) / TILE;
+    const int t1 = (end + TILE - 1) / TILE;
+    const int first = row0 + wave * 32, last = first + 31;
+    const float sl2 = a.scale * 1.44269504088896340736f;
+    stage<DP>(kp, a.k_t, t0 * TILE, s.len, a.D, lds[0]);
+    stage<DP>(vp, a.v_t, t0 * TILE, s.len, a.D, lds[1]);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int kv0 = t * TILE;
+      char* kt = lds[(t - t0) & 1 ? 2 : 0];
+      char* vt = lds[(t - t0) & 1 ? 3 : 1];
+      if (t + 1 < t1) {
+        stage<DP>(kp, a.k_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 0 : 2]);
+        stage<DP>(vp, a.v_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 1 : 3]);
+      }
+      if ((!CAUSAL || kv0 <= last) && first < s.len &&
+          (!a.window || kv0 + TILE > first - a.window + 1)) {
+        const bool edge = kv0 + TILE > s.len ||
+                          (CAUSAL && kv0 + TILE - 1 > first) ||
+                          (a.window && kv0 <= last - a.window);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            sc = E::mfma(rows_of<DP>(kt, 32 * kb, kk, lane), q[kk], sc);
+            dp = E::mfma(rows_of<DP>(vt, 32 * kb, kk, lane), dO[kk], dp);
+          }
+          float ds[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p = exp2f(sc[i] * sl2 - lse);
+            if (edge) {
+              const int key = kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) +
+                              i % 4;
+              bool seen = key < s.len;
+              if (CAUSAL) seen &= key <= row;
+              if (a.window) seen &= key > row - a.window;
+              if (!seen) p = 0.f;
+            }
+            // dS is rounded to the type of k, which the product needs
+            ds[i] = p * (dp[i] * a.scale - dr);
+          }
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const short8 b = E::pack(ds + 8 * ks);
+#pragma unroll
+            for (int f = 0; f < DP / 32; ++f)
+              dq[f] = E::mfma(cols_of<DP>(kt, 32 * kb + 16 * ks, f, lane), b,
+                              dq[f]);
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if (row < s.rows)
+    put_rows<E, DP>(a.dq + (at * a.H + head) * a.D, live, a.D, lane, 1.f, dq);
+}
+
+// ---- backward: dK and dV -----------------------------------------------
+// A block owns 128 keys of one kv head and goes through the query tiles of
+// all its heads: shared heads add up in registers, in a fixed order.
+
+template <class E, int DP, bool CAUSAL>
+__global__ __launch_bounds__(NTH, 1) void packed_bwd_kv_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][TILE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rep = a.H / a.HK;
+  int kvh, slot, sub, row0;
+  Seq s;
+  if (!unit_of(a, 1, kvh, slot, sub)) return;
+  if (!tile_of<OWN>(a, slot, s, row0)) return;
+  const int key = row0 + wave * 32 + (lane & 31);
+  const bool live = key < s.len;
+  const long at = s.begin + key;
+
+  float16v dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int f = 0; f < DP / 32; ++f) dk[f] = dv[f] = (float16v)(0.f);
+
+  if (row0 < s.len) {
+    short8 k[DP / 16], v[DP / 16];
+    own_rows<DP>(a.k + at * a.k_t + kvh * a.k_h, live, a.D, lane, k);
+    own_rows<DP>(a.v + at * a.v_t + kvh * a.v_h, live, a.D, lane, v);
+    const int t0 = CAUSAL ? row0 / TILE : 0;
+    int end = s.len;
+    if (a.window) end = min((long)end, (long)row0 + OWN - 1 + a.window);
+    const int tiles = (end + TILE - 1) / TILE - t0;
+    const int first = row0 + wave * 32, last = first + 31;
+    const float sl2 = a.scale * 1.44269504088896340736f;
+    auto fetch = [&](int n, int buf) {
+      const int head = kvh * rep + n / tiles, q0 = (t0 + n % tiles) * TILE;
+      stage<DP>(a.q + (long)s.begin * a.q_t + head * a.q_h, a.q_t, q0, s.len,
+                a.D, lds[2 * buf]);
+      stage<DP>(a.dout + (long)s.begin * a.d_t + head * a.d_h, a.d_t, q0,
+                s.len, a.D, lds[2 * buf + 1]);
+      if (threadIdx.x < TILE) {
+        const int row = q0 + threadIdx.x;
+        const long e = (long)head * a.T + s.begin + row;
+        const bool ok = row < s.len;
+        stat[buf][0][threadIdx.x] = ok ? a.lse[e] : INFINITY;
+        stat[buf][1][threadIdx.x] = ok ? a.drow[e] : 0.f;
+      }
+    };
+    fetch(0, 0);
+    __syncthreads();
+    for (int n = 0; n < rep * tiles; ++n) {
+      const int buf = n & 1, q0 = (t0 + n % tiles) * TILE;
+      if (n + 1 < rep * tiles) fetch(n + 1, buf ^ 1);
+      const char *qt = lds[2 * buf], *dt = lds[2 * buf + 1];
+      if ((!CAUSAL || q0 + TILE > first) && first < s.len &&
+          (!a.window || q0 <= last + a.window - 1)) {
+        const bool edge = (CAUSAL && q0 < last) ||
+                          (a.window && q0 + TILE - 1 >= first + a.window);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            sc = E::mfma(rows_of<DP>(qt, 32 * qb, kk, lane), k[kk], sc);
+            dp = E::mfma(rows_of<DP>(dt, 32 * qb, kk, lane), v[kk], dp);
+          }
+          float p[16], ds[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = 32 * qb + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+            p[i] = exp2f(sc[i] * sl2 - stat[buf][0][r]);
+            if (edge) {
+              bool seen = true;
+              if (CAUSAL) seen &= key <= q0 + r;
+              if (a.window) seen &= key > q0 + r - a.window;
+              if (!seen) p[i] = 0.f;
+            }
+            ds[i] = p[i] * (dp[i] * a.scale - stat[buf][1][r]);
+          }
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const short8 pb = E::pack(p + 8 * ks), sb = E::pack(ds + 8 * ks);
+#pragma unroll
+            for (int f = 0; f < DP / 32; ++f) {
+              dv[f] = E::mfma(cols_of<DP>(dt, 32 * qb + 16 * ks, f, lane), pb,
+                              dv[f]);
+              dk[f] = E::mfma(cols_of<DP>(qt, 32 * qb + 16 * ks, f, lane), sb,
+                              dk[f]);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if (key < s.rows) {
+    put_rows<E, DP>(a.dk + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dk);
+    put_rows<E, DP>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dv);
+  }
+}
+
+// ---- host --------------------------------------------------------------
+
+bool rows_aligned(const torch::Tensor& t) {
+  return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+         (size_t)t.data_ptr() % 16 == 0;
+}
+
+Args args_of(const torch::Tensor& q, const torch::Tensor& k,
+             const torch::Tensor& v, const torch::Tensor& cu,
+             const c10::optional<torch::Tensor>& lengths, int64_t window,
+             double scale) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3 &&
+              k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+              k.size(2) == q.size(2),
+              "attn_packed: q [T,H,D], k and v [T,HK,D] on the GPU");
+  const auto st = q.scalar_type();
+  TORCH_CHECK((st == torch::kBFloat16 || st == torch::kHalf) &&
+              k.scalar_type() == st && v.scalar_type() == st,
+              "attn_packed: q, k and v must all be bf16 or fp16");
+  TORCH_CHECK(k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0,
+              "attn_packed: kv heads must divide q heads");
+  TORCH_CHECK(q.size(2) % 8 == 0 && q.size(2) >= 8 && q.size(2) <= 128,
+              "attn_packed: D must be a multiple of 8, at most 128");
+  TORCH_CHECK(rows_aligned(q) && rows_aligned(k) && rows_aligned(v),
+              "attn_packed: rows must be dense and 16-byte aligned");
+  TORCH_CHECK(q.size(0) < (1L << 30), "attn_packed: too many rows");
+  TORCH_CHECK(cu.dim() == 1 && cu.size(0) >= 2 && cu.is_contiguous() &&
+              cu.scalar_type() == torch::kInt,
+              "attn_packed: cu_seqlens must be int32 [sequences + 1]");
+  for (const auto& x : {k, v, cu})
+    TORCH_CHECK(x.device() == q.device(),
+                "attn_packed: all tensors must be on one device");
+  if (lengths.has_value())
+    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == cu.size(0) - 1 &&
+                lengths->is_contiguous() &&
+                lengths->scalar_type() == torch::kInt &&
+                lengths->device() == q.device(),
+                "attn_packed: lengths must be int32 [sequences]");
+  Args a = {};
+  a.q = (const short*)q.data_ptr();
+  a.k = (const short*)k.data_ptr();
+  a.v = (const short*)v.data_ptr();
+  a.q_t = q.stride(0); a.q_h = q.stride(1);
+  a.k_t = k.stride(0); a.k_h = k.stride(1);
+  a.v_t = v.stride(0); a.v_h = v.stride(1);
+  a.cu = cu.data_ptr<int>();
+  a.lengths = lengths ? lengths->data_ptr<int>() : nullptr;
+  a.T = (int)q.size(0);
+  a.B = (int)cu.size(0) - 1;
+  a.H = (int)q.size(1);
+  a.HK = (int)k.size(1);
+  a.D = (int)q.size(2);
+  a.window = (int)std::min<int64_t>(window, a.T);
+  a.scale = (float)scale;
+  const long units = ((long)a.T / OWN + a.B + 1) * a.HK;
+  TORCH_CHECK(units * (a.H / a.HK) < (1L << 30),
+              "attn_packed: too many rows and heads");
+  a.units = (int)units;
+  return a;
+}
+
+#define PACKED_LAUNCH(KERNEL, REP)                                          \
+  do {                                                                      \
+    const dim3 grid((a.units + 7) / 8 * 8 * (REP)), block(NTH);             \
+    const auto st = stream.stream();                                        \
+    if (bf && wide && causal)                                               \
+      hipLaunchKernelGGL((KERNEL<BF, 128, true>), grid, block, 0, st, a);   \
+    else if (bf && wide)                                                    \
+      hipLaunchKernelGGL((KERNEL<BF, 128, false>), grid, block, 0, st, a);  \
+    else if (bf && causal)                                                  \
+      hipLaunchKernelGGL((KERNEL<BF, 64, true>), grid, block, 0, st, a);    \
+    else if (bf)                                                            \
+      hipLaunchKernelGGL((KERNEL<BF, 64, false>), grid, block, 0, st, a);   \
+    else if (wide && causal)                                                \
+      hipLaunchKernelGGL((KERNEL<FH, 128, true>), grid, block, 0, st, a);   \
+    else if (wide)                                                          \
+      hipLaunchKernelGGL((KERNEL<FH, 128, false>), grid, block, 0, st, a);  \
+    else if (causal)                                                        \
+      hipLaunchKernelGGL((KERNEL<FH, 64, true>), grid, block, 0, st, a);    \
+    else                                                                    \
+      hipLaunchKernelGGL((KERNEL<FH, 64, false>), grid, block, 0, st, a);   \
+  } while (0)
+
+}  // namespace
+
+// {o [T,H,D], lse [H,T] in units of log 2, +inf for rows without tokens}
+std::vector<torch::Tensor> attn_packed_fwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu,
+    c10::optional<torch::Tensor> lengths, bool causal, int64_t window,
+    double scale) {
+  Args a = args_of(q, k, v, cu, lengths, window, scale);
+  TORCH_CHECK(window >= 0 && (window == 0 || causal),
+              "attn_packed: a window needs a causal mask");
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto o = torch::empty(q.sizes(), q.options());
+  auto lse = torch::empty({a.H, a.T}, q.options().dtype(torch::kFloat32));
+  if (a.T == 0) return {o, lse};
+  a.out = (short*)o.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  auto stream = c10::cuda::getCurrentCUDAStream();
+  const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
+  PACKED_LAUNCH(packed_fwd_kernel, a.H / a.HK);
+  HIP_CHECK_LAST();
+  return {o, lse};
+}
+
+// {dq, dk, dv}, contiguous
+std::vector<torch::Tensor> attn_packed_bwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o,
+    torch::Tensor dout, torch::Tensor lse, torch::Tensor cu,
+    c10::optional<torch::Tensor> lengths, bool causal, int64_t window,
+    double scale) {
+  Args a = args_of(q, k, v, cu, lengths, window, scale);
+  TORCH_CHECK(dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&
+              o.is_contiguous() && dout.scalar_type() == q.scalar_type() &&
+              o.scalar_type() == q.scalar_type() && rows_aligned(dout) &&
+              dout.device() == q.device(),
+              "attn_packed: o and dout must be like q, dout's rows dense and "
+              "16-byte aligned");
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto dq = torch::empty(q.sizes(), q.options());
+  auto dk = torch::empty(k.sizes(), k.options());
+  auto dv = torch::empty(v.sizes(), v.options());
+  if (a.T == 0) return {dq, dk, dv};
+  auto drow = torch::empty_like(lse);
+  a.o = (const short*)o.data_ptr();
+  a.dout = (const short*)dout.data_ptr();
+  a.d_t = dout.stride(0);
+  a.d_h = dout.stride(1);
+  a.dq = (short*)dq.data_ptr();
+  a.dk = (short*)dk.data_ptr();
+  a.dv = (short*)dv.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  a.drow = drow.data_ptr<float>();
+  auto stream = c10::cuda::getCurrentCUDAStream();
+  const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
+  PACKED_LAUNCH(packed_bwd_q_kernel, a.H / a.HK);
+  PACKED_LAUNCH(packed_bwd_kv_kernel, 1);
+  HIP_CHECK_LAST();
+  return {dq, dk, dv};
+}

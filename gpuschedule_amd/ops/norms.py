@@ -6,6 +6,8 @@ same math via plain fp32 torch ops under autograd.
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.nn as nn
 
@@ -102,3 +104,115 @@ class FusedRMSNorm(nn.Module):
 
     def extra_repr(self):
         return f"{self.dim}, eps={self.eps}"
+
+
+class _BlockNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, x, post_weight, pre_weight, gate, alpha, eps):
+        ext = get_ext(required=True)
+        train = any(ctx.needs_input_grad)
+        n, s, r1, r2 = ext.block_norm_fwd(h, x, post_weight, pre_weight,
+                                          gate, alpha, eps, train)
+        # the sum is computed again in backward, from h and x
+        ctx.save_for_backward(h, x, post_weight, pre_weight, gate, r1, r2)
+        ctx.alpha = alpha
+        return n, s
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dn, ds):
+        ext = get_ext(required=True)
+        h, x, w1, w2, gate, r1, r2 = ctx.saved_tensors
+        dh, dx, dw1, dw2, dg = ext.block_norm_bwd(
+            dn.contiguous(), ds.contiguous(), h, x, w1, w2, gate, r1, r2,
+            ctx.alpha)
+        return (dh, dx, dw1, dw2, dg if gate is not None else None, None,
+                None)
+
+
+def fused_block_norm(h: torch.Tensor, x: torch.Tensor,
+                     post_weight: torch.Tensor, pre_weight: torch.Tensor,
+                     gate: Optional[torch.Tensor] = None,
+                     residual_scale: float = 1.0, eps: float = 1e-6):
+    """What stands between two residual blocks, in one pass each way:
+
+        s = residual_scale * x + gate * rmsnorm(h) * post_weight
+        n = rmsnorm(s) * pre_weight
+
+    ``h`` [..., D] is a block's output, ``x`` [..., D] the residual
+    stream before it.  Returns ``(n, s)``: the next block's input and
+    the stream behind the sum (``FusedRMSNorm``'s ``return_sum`` order).
+
+    ``gate``: ``[D]`` for all rows, ``[h.shape[0], D]`` for one gate row
+    for each index of h's first dimension (a sequence of a batch), or
+    h's own shape; None is 1.  All tensors share one type (bf16, fp16 or
+    fp32) and device; D is at most 16384.  Statistics and sums are fp32,
+    ``n`` is computed from the sum before that is rounded.  Inputs that
+    are not contiguous are copied."""
+    D = h.shape[-1] if h.dim() else 0
+    if x.shape != h.shape:
+        raise ValueError(f"fused_block_norm: x is {tuple(x.shape)}, "
+                         f"h is {tuple(h.shape)}")
+    for name, w in (("post_weight", post_weight),
+                    ("pre_weight", pre_weight)):
+        if w.shape != (D,):
+            raise ValueError(f"fused_block_norm: {name} must be [{D}], "
+                             f"got {tuple(w.shape)}")
+    for t in (x, post_weight, pre_weight, gate):
+        if t is not None and (t.dtype != h.dtype or t.device != h.device):
+            raise ValueError("fused_block_norm: all tensors must have h's "
+                             "type and device")
+    if not 1 <= D <= 16384:
+        raise ValueError(f"fused_block_norm: D must be 1 to 16384, got {D}")
+    if h.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"fused_block_norm: bf16, fp16 or fp32 only, "
+                         f"got {h.dtype}")
+    if gate is not None and gate.shape != (D,) and gate.shape != h.shape \
+            and gate.shape != (h.shape[0], D):
+        raise ValueError(f"fused_block_norm: gate {tuple(gate.shape)} is "
+                         f"none of [D], [h.shape[0], D] and h's shape")
+    if not h.is_cuda:
+        g = 1.0
+        if gate is not None:
+            g = gate.float()
+            if gate.shape != h.shape and gate.dim() == 2:
+                g = g.view(h.shape[0], *[1] * (h.dim() - 2), D)
+        hf, xf = h.float(), x.float()
+        z = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps)
+        s = residual_scale * xf + g * (z * post_weight.float())
+        n = s * torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + eps)
+        return (n * pre_weight.float()).to(h.dtype), s.to(h.dtype)
+    if gate is not None:
+        gate = gate.reshape(-1, D).contiguous()
+        if h.numel() == 0:
+            gate = None
+    return _BlockNormFn.apply(h.contiguous(), x.contiguous(),
+                              post_weight.contiguous(),
+                              pre_weight.contiguous(), gate,
+                              float(residual_scale), float(eps))
+
+
+class FusedBlockNorm(nn.Module):
+    """:func:`fused_block_norm` with its weights.  ``gated=True`` adds a
+    learned gate [D] that begins at ``gate_init``; a gate given to
+    ``forward`` takes its place."""
+
+    def __init__(self, dim: int, residual_scale: float = 1.0,
+                 gated: bool = False, gate_init: float = 1.0,
+                 eps: float = 1e-6):
+        super().__init__()
+        self.dim, self.eps = dim, eps
+        self.residual_scale = residual_scale
+        self.post_weight = nn.Parameter(torch.ones(dim))
+        self.pre_weight = nn.Parameter(torch.ones(dim))
+        self.gate = (nn.Parameter(torch.full((dim,), float(gate_init)))
+                     if gated else None)
+
+    def forward(self, h, x, gate=None):
+        return fused_block_norm(h, x, self.post_weight, self.pre_weight,
+                                self.gate if gate is None else gate,
+                                self.residual_scale, self.eps)
+
+    def extra_repr(self):
+        return (f"{self.dim}, residual_scale={self.residual_scale}, "
+                f"gated={self.gate is not None}, eps={self.eps}")

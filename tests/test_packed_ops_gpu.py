@@ -1,0 +1,845 @@
+"""Packed attention, rotary on axes, block norm and gradient clipping
+against plain 64-bit implementations.
+
+Tolerances are bounds, element by element.  u = eps / 2 of the type is the
+largest relative error of one rounding; fp16 adds 2^-25, half its smallest
+step, where values are subnormal.  32-bit arithmetic is allowed the small
+power of two that each test derives."""
+import itertools
+import math
+
+import pytest
+import torch
+
+from gpuschedule_amd.ops import (FusedAdamW, FusedBlockNorm, clip_grad_norm_,
+                                 flash_attention_packed, fused_block_norm,
+                                 fused_rope_axes, grad_norm)
+
+pytestmark = pytest.mark.gpu
+
+BF, FH, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def subnormal(dtype):
+    return 2.0 ** -25 if dtype == FH else 0.0
+
+
+def within(got, want, tol, what):
+    got = got.double()
+    if not got.numel():
+        return
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = ((got - want).abs() - tol).max().item()
+    assert over <= 0, f"{what}: {over:.3g} over its bound"
+
+
+def normal(shape, dtype, seed, scale=1.0, shift=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(shape, device="cuda", generator=g) * scale + shift
+    return x.to(dtype)
+
+
+# ---- packed attention ------------------------------------------------------
+
+def seen_of(spans, lengths, rows, causal, window):
+    seq = torch.full((rows,), -1)
+    at = 0
+    for i, n in enumerate(spans):
+        used = n if lengths is None else lengths[i]
+        seq[at:at + used] = i
+        at += n
+    i = torch.arange(rows)
+    seen = (seq[:, None] == seq) & (seq >= 0)[:, None]
+    if causal:
+        seen &= i <= i[:, None]
+    if window:
+        seen &= i > i[:, None] - window
+    return seen.cuda()
+
+
+def oracle(q, k, v, do, seen, scale):
+    """64-bit o, dq, dk, dv, and how far each element may be off."""
+    u, sub = unit(q.dtype), subnormal(q.dtype)
+    slack = 2.0 ** -14   # of 32-bit scores, exp2 and sums where |s| < 32:
+    #                      s is off by some 2^-24 of the 32 to 100 that its
+    #                      terms add up to, and p by that relative; larger
+    #                      scores are off by as much more
+    rep = q.shape[1] // k.shape[1]
+    q, k, v, do = (x.detach().double().transpose(0, 1)
+                   for x in (q, k, v, do))
+    kr, vr = (x.repeat_interleave(rep, 0) for x in (k, v))
+    s = (q @ kr.transpose(-1, -2)) * scale
+    slack *= max(1.0, s.abs().max().item() / 32) if s.numel() else 1.0
+    s = s.masked_fill(~seen, -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)   # rows that see nothing
+    o = p @ vr
+    mass = p @ vr.abs()
+    many = seen.double() @ vr.abs()
+    tol_o = u * (mass + o.abs()) + slack * mass + sub * (many + 1)
+    dp = do @ vr.transpose(-1, -2)
+    drow = (do * o).sum(-1, keepdim=True)
+    ds = scale * p * (dp - drow)
+    # D is taken from the rounded o
+    off_d = (do.abs() * tol_o).sum(-1, keepdim=True)
+    off_ds = scale * p * (off_d + slack * (do.abs() @ vr.abs().transpose(
+        -1, -2) + drow.abs() + off_d)) + (u + slack) * ds.abs() + sub * seen
+    dq, dk, dv = ds @ kr, ds.transpose(-1, -2) @ q, p.transpose(-1, -2) @ do
+    tol_q = off_ds @ kr.abs() + u * dq.abs() + sub
+    tol_k = off_ds.transpose(-1, -2) @ q.abs()
+    tol_v = (u + slack) * (p.transpose(-1, -2) @ do.abs()) \
+        + sub * (seen.double().t() @ do.abs())
+
+    def group(x):
+        return x.unflatten(0, (-1, rep)).sum(1)
+
+    dk, dv = group(dk), group(dv)
+    tol_k = group(tol_k) + u * dk.abs() + sub
+    tol_v = group(tol_v) + u * dv.abs() + sub
+    # sums of many terms that cancel: 32-bit products and sums again
+    return [(a.transpose(0, 1), t.transpose(0, 1)) for a, t in (
+        (o, tol_o), (dq, tol_q * (1 + slack)), (dk, tol_k * (1 + slack)),
+        (dv, tol_v * (1 + slack)))]
+
+
+def cu_of(spans):
+    return torch.tensor([0] + list(itertools.accumulate(spans)),
+                        dtype=torch.int32, device="cuda")
+
+
+def ints(values):
+    return None if values is None else torch.tensor(
+        values, dtype=torch.int32, device="cuda")
+
+
+def qkv_of(rows, H, HK, D, dtype, seed, scale=1.0):
+    """Slices of one projection, as leaves."""
+    x = normal((rows, (H + 2 * HK) * D), dtype, seed, scale)
+    q, k, v = x.split([H * D, HK * D, HK * D], -1)
+    return [t.unflatten(-1, (-1, D)).detach().requires_grad_()
+            for t in (q, k, v)]
+
+
+def check_attention(spans, rows, H, HK, D, dtype, lengths=None, causal=False,
+                    window=None, scale=None, size=1.0, seed=0):
+    q, k, v = qkv_of(rows, H, HK, D, dtype, seed, size)
+    do = normal((rows, H, D), dtype, seed + 1)
+    o = flash_attention_packed(q, k, v, cu_of(spans), ints(lengths), causal,
+                               window, scale)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    seen = seen_of(spans, lengths, rows, causal, window)
+    want = oracle(q, k, v, do, seen, scale or 1 / math.sqrt(D))
+    for got, (w, tol), name in zip((o,) + grads, want,
+                                   ("o", "dq", "dk", "dv")):
+        within(got, w, tol, name)
+        if not got[0].numel():
+            continue
+        dead = ~seen.any(1)
+        assert (got[dead] == 0).all(), f"{name}: padding rows"
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129,
+                               255, 257, 640])
+def test_attention_one_sequence(n, causal):
+    check_attention([n], n, 2, 1, 64, BF, causal=causal, seed=n)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("D", [8, 16, 40, 64, 72, 96, 120, 128])
+def test_attention_head_sizes(D, dtype):
+    check_attention([130, 1, 77], 208, 3, 3, D, dtype, causal=True, seed=D)
+    check_attention([130, 1, 77], 208, 2, 1, D, dtype, seed=D)
+
+
+@pytest.mark.parametrize("H,HK", [(1, 1), (4, 4), (6, 2), (8, 1), (12, 3),
+                                  (5, 5)])
+def test_attention_shared_heads(H, HK):
+    check_attention([200, 100], 300, H, HK, 64, BF, causal=True, seed=H)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("spans,rows", [
+    ([0, 5, 0, 0, 127, 1, 0], 133),       # empty sequences
+    ([0], 4),                             # no tokens at all
+    ([128, 128, 128], 384),               # tiles end with sequences
+    ([100], 357),                         # rows behind the last sequence
+    ([1] * 200, 200),                     # one token each
+    ([127, 129, 63, 65, 500], 900),
+])
+def test_attention_spans(spans, rows, causal):
+    check_attention(spans, rows, 4, 2, 64, BF, causal=causal, seed=rows)
+    check_attention(spans, rows, 2, 2, 128, FH, causal=causal, seed=rows)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_padded_batch(causal):
+    check_attention([150] * 5, 750, 4, 4, 64, BF,
+                    lengths=[150, 0, 1, 128, 77], causal=causal)
+    check_attention([128, 40, 64], 300, 4, 2, 128, BF,
+                    lengths=[0, 40, 3], causal=causal)
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 128, 200, 10 ** 9])
+def test_attention_window(window):
+    check_attention([333, 70], 403, 2, 1, 64, BF, causal=True, window=window,
+                    seed=window % 97)
+    check_attention([300, 5], 310, 2, 2, 128, FH, causal=True, window=window,
+                    lengths=[290, 4], seed=window % 97)
+
+
+def test_attention_long():
+    # 4,1k rows: many tiles in a row, maxima that move on
+    check_attention([4100], 4100, 1, 1, 128, BF, causal=True, seed=3)
+    check_attention([1500, 2600], 4100, 1, 1, 64, FH, seed=4)
+
+
+def test_attention_sharp_scores():
+    # scores of about +-25: one key takes nearly all of a row, and maxima
+    # jump by more than the exponent of fp16 holds
+    check_attention([700], 700, 2, 1, 64, BF, causal=True, scale=1.0,
+                    size=1.7, seed=5)
+    check_attention([700], 700, 2, 1, 64, FH, scale=1.0, size=1.7, seed=6)
+
+
+def test_attention_late_maximum():
+    # the last keys of the first rows are by far the largest
+    q, k, v = qkv_of(320, 1, 1, 64, BF, 9)
+    with torch.no_grad():
+        q[:64] = q[:64].abs()
+        k[300:] = 4.0
+    do = normal((320, 1, 64), BF, 10)
+    o = flash_attention_packed(q, k, v, cu_of([320]), scale=0.1)
+    got = (o,) + torch.autograd.grad(o, (q, k, v), do)
+    seen = torch.ones(320, 320, dtype=torch.bool, device="cuda")
+    for g, (w, tol) in zip(got, oracle(q, k, v, do, seen, 0.1)):
+        within(g, w, tol, "late maximum")
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_keeps_what_is_not_finite_apart(bad):
+    """Rows of padding, of another sequence or behind the last one may hold
+    anything; a sequence's own end tile does not let it in."""
+    spans, lengths, rows = [100, 90, 70], [100, 60, 70], 300
+    q, k, v = qkv_of(rows, 2, 1, 64, BF, 11)
+    do = normal((rows, 2, 64), BF, 12)
+    with torch.no_grad():
+        for t in (q, k, v, do):
+            t[160:190] = bad          # padding of the second
+            t[260:] = bad             # behind the last
+            t[190:260] = bad          # all of the third
+    o = flash_attention_packed(q, k, v, cu_of(spans), ints(lengths), True)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    with torch.no_grad():
+        for t in (q, k, v, do):
+            t[160:] = 0
+    seen = seen_of(spans, [100, 60, 0], rows, True, None)
+    want = oracle(q, k, v, do, seen, 1 / 8)
+    for got, (w, tol) in zip((o,) + grads, want):
+        within(got[:160], w[:160], tol[:160], "beside bad rows")
+        assert (got[160:190] == 0).all() and (got[260:] == 0).all()
+
+
+def test_attention_layouts():
+    """Values do not depend on strides, and odd ones are copied."""
+    T, H, HK, D = 150, 4, 2, 64
+    q, k, v = (normal((T, n, D), BF, i) for i, n in enumerate((H, HK, HK)))
+    cu = cu_of([100, 50])
+    want = flash_attention_packed(q, k, v, cu, causal=True)
+    per_head = [t.transpose(0, 1).contiguous().transpose(0, 1)
+                for t in (q, k, v)]
+    apart = [torch.stack([t, t], -1)[..., 0] for t in (q, k, v)]
+    odd = []
+    for t in (q, k, v):      # rows that begin 2 bytes past a line
+        room = torch.zeros(T * t.shape[1] * (D + 1) + 1, device="cuda",
+                           dtype=BF)
+        w = room[1:].view(T, t.shape[1], D + 1)[..., :D]
+        w.copy_(t)
+        odd.append(w)
+    for x in (per_head, apart, odd):
+        assert torch.equal(flash_attention_packed(*x, cu, causal=True), want)
+    # a gradient that is one row for all
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = flash_attention_packed(*leaves, cu, causal=True)
+    a = torch.autograd.grad(o, leaves, torch.ones((), device="cuda",
+                                                  dtype=BF).expand_as(o),
+                            retain_graph=True)
+    b = torch.autograd.grad(o, leaves, torch.ones_like(o))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_attention_is_the_same_every_time():
+    q, k, v = qkv_of(2000, 8, 2, 128, BF, 21)
+    do = normal((2000, 8, 128), BF, 22)
+    first = None
+    for _ in range(4):
+        o = flash_attention_packed(q, k, v, cu_of([700, 1300]), causal=True)
+        got = (o.detach(),) + torch.autograd.grad(o, (q, k, v), do)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_attention_bad_cu_stays_inside():
+    """Values of cu_seqlens and lengths that make no sense touch nothing
+    else and end."""
+    q, k, v = qkv_of(256, 2, 1, 64, BF, 31)
+    for cu, lengths in (([0, 1000], None), ([0, 200, 100, 256], None),
+                        ([-5, 300], [7]), ([0, 100, 256], [-3, 99999]),
+                        ([256, 0], None)):
+        o = flash_attention_packed(q, k, v, ints(cu), ints(lengths), True)
+        torch.autograd.grad(o.sum(), (q, k, v))
+        torch.cuda.synchronize()
+    assert all(torch.isfinite(t).all() for t in (q, k, v))
+
+
+def test_attention_agrees_with_differences():
+    """The gradients along a direction against differences of the 64-bit
+    forward pass (h^2 error about 1e-6 of the second derivative)."""
+    T, spans = 96, [60, 36]
+    q, k, v = qkv_of(T, 2, 1, 64, FH, 41)
+    do = normal((T, 2, 64), FH, 42)
+    o = flash_attention_packed(q, k, v, cu_of(spans), causal=True)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    seen = seen_of(spans, None, T, True, None)
+    bounds = oracle(q, k, v, do, seen, 1 / 8)[1:]
+
+    def forward(q, k, v):
+        k, v = (x.repeat_interleave(2, 1) for x in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q, k) / 8
+        p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        return (torch.einsum("hqk,khd->qhd", p, v) * do.double()).sum()
+
+    base = [x.detach().double() for x in (q, k, v)]
+    for n in range(3):
+        d = normal(base[n].shape, torch.float64, 50 + n)
+        h = 1e-3
+        up, down = (list(base) for _ in range(2))
+        up[n], down[n] = base[n] + h * d, base[n] - h * d
+        slope = (forward(*up) - forward(*down)) / (2 * h)
+        along = (grads[n].double() * d).sum()
+        room = (bounds[n][1] * d.abs()).sum() + 1e-4 * d.abs().sum()
+        assert (slope - along).abs() <= room
+
+
+# ---- rotary on axes --------------------------------------------------------
+
+def rope_tables(places, half, base=1e4):
+    inv = base ** (-torch.arange(half, dtype=torch.float64) / half)
+    angle = torch.outer(torch.arange(places, dtype=torch.float64), inv)
+    return angle.cos().float().cuda(), angle.sin().float().cuda()
+
+
+def check_rope(q, k, positions, cos, sin, sections, back=True):
+    half = cos.shape[1]
+    axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    at = positions.long()[axis].t()
+    j = torch.arange(half, device="cuda")
+    c, s = (t[at, j].double()[:, None] for t in (cos, sin))
+    u, sub = unit(q.dtype), subnormal(q.dtype)
+
+    def turned(x, s):
+        x = x.detach().double()
+        a, b = x[..., :half], x[..., half:2 * half]
+        y = torch.cat([a * c - b * s, b * c + a * s, x[..., 2 * half:]], -1)
+        m = (a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()
+        # three 32-bit roundings of the terms, one of the result; what
+        # passes through stays as it is
+        tol = torch.cat([*m, torch.zeros_like(x[..., 2 * half:])], -1)
+        tol = 3 * 2.0 ** -24 * tol
+        tol[..., :2 * half] += (u * y.abs() + sub)[..., :2 * half]
+        return y, tol
+
+    out = fused_rope_axes(q, k, positions, cos, sin, sections)
+    for got, x in zip(out, (q, k)):
+        within(got, *turned(x, s), "turned")
+        assert got.is_contiguous()
+    if back:
+        g = [normal(x.shape, x.dtype, 7 + i) for i, x in enumerate((q, k))]
+        for got, x in zip(torch.autograd.grad(out, (q, k), g), g):
+            within(got, *turned(x, -s), "gradient")
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FP])
+@pytest.mark.parametrize("T,H,HK,D,sections", [
+    (1, 1, 1, 2, [1]),
+    (3, 4, 2, 64, [32]),
+    (37, 8, 8, 128, [16, 24, 24]),
+    (129, 5, 1, 80, [7, 33]),            # runs that cross axes
+    (65, 3, 3, 72, [1, 2, 3, 30]),       # half a run at the end
+    (40, 12, 4, 128, [10, 6]),           # most values pass through
+    (21, 2, 1, 70, [11, 11]),            # odd rows: 2-byte alignment
+    (700, 9, 3, 256, [40, 44, 44]),
+])
+def test_rope_axes(T, H, HK, D, sections, dtype):
+    q, k, _ = qkv_of(T, H, HK, D, dtype, T)
+    cos, sin = rope_tables(97, sum(sections))
+    for wide in (torch.int64, torch.int32):
+        pos = torch.randint(0, 97, (len(sections), T), device="cuda",
+                            dtype=wide)
+        check_rope(q, k, pos, cos, sin, sections)
+
+
+def test_rope_is_the_dense_rope_on_one_axis():
+    from gpuschedule_amd.ops.elementwise import fused_rope
+    B, H, S, D = 2, 4, 50, 64
+    x = normal((B, S, H, D), BF, 1)
+    cos, sin = rope_tables(S, D // 2)
+    pos = torch.arange(S, device="cuda").repeat(B)[None]
+    flat = x.view(B * S, H, D)
+    got, _ = fused_rope_axes(flat, flat, pos, cos, sin, [D // 2])
+    want = fused_rope(x.transpose(1, 2), cos, sin).transpose(1, 2)
+    assert torch.equal(got.view(B, S, H, D), want)
+
+
+def test_rope_far_and_bad_positions():
+    D, places = 64, 200_000
+    cos, sin = rope_tables(places, 32)
+    q, k, _ = qkv_of(4, 2, 1, D, BF, 2)
+    pos = torch.tensor([[0, places - 1, 77_777, 131_072]], device="cuda")
+    check_rope(q, k, pos, cos, sin, [32], back=False)
+    pos = torch.tensor([[0, places, -1, 1 << 40], [1, 2, 3, 4]],
+                       device="cuda")
+    y, _ = fused_rope_axes(q, k, pos, cos, sin, [8, 24])
+    y = y.unflatten(-1, (2, 32))
+    assert y[1:, :, :, :8].isnan().all()      # those tokens, that axis
+    assert not y[0].isnan().any() and not y[..., 8:].isnan().any()
+
+
+def test_rope_odd_gradients_and_nothing():
+    cos, sin = rope_tables(9, 16)
+    pos = torch.zeros(1, 5, dtype=torch.int64, device="cuda")
+    q, k, _ = qkv_of(5, 3, 1, 40, BF, 3)
+    out = fused_rope_axes(q, k, pos, cos, sin, [16])
+    one = torch.ones((), device="cuda", dtype=BF)
+    a = torch.autograd.grad(out, (q, k), [one.expand_as(t) for t in out],
+                            retain_graph=True)
+    b = torch.autograd.grad(out, (q, k), [torch.ones_like(t) for t in out],
+                            retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    (c,) = torch.autograd.grad(out[0], q, torch.ones_like(out[0]))
+    assert torch.equal(c, b[0])               # k unused: its gradient is 0
+    empty = q[:0], k[:0], pos[:, :0]
+    assert fused_rope_axes(*empty, cos, sin, [16])[0].shape == (0, 3, 40)
+
+
+# ---- block norm ------------------------------------------------------------
+
+def check_block_norm(shape, dtype, gate, alpha=1.0, eps=1e-6, seed=0):
+    D = shape[-1]
+    h, x = normal(shape, dtype, seed, 0.7), normal(shape, dtype, seed + 1, 2)
+    w1, w2 = (normal((D,), dtype, seed + i, 0.2, 1.0) for i in (2, 3))
+    g = None if gate is None else normal(gate, dtype, seed + 4, 0.5, 0.3)
+    dn, ds = normal(shape, dtype, seed + 5), normal(shape, dtype, seed + 6)
+    leaves = [t.requires_grad_() for t in (h, x, w1, w2, g) if t is not None]
+    n, s = fused_block_norm(h, x, w1, w2, g, alpha, eps)
+    grads = torch.autograd.grad((n, s), leaves, (dn, ds))
+
+    u, sub = unit(dtype), subnormal(dtype)
+    # a mean of D values: a lane adds 16, lanes and waves 10 more, and some
+    # ten products follow: under 2^-19 relative; a difference of such terms
+    # is off by that of their sizes, twice over in backward
+    slack, back = 2.0 ** -17, 2.0 ** -15
+    hd, xd, a, b = (t.detach().double() for t in (h, x, w1, w2))
+    gd = 1.0 if g is None else g.detach().double()
+    if g is not None and g.dim() == 2 and len(shape) != 2:
+        gd = gd.view(shape[0], *[1] * (len(shape) - 2), D)
+    r1 = (hd.square().mean(-1, keepdim=True) + eps).rsqrt()
+    hh = hd * r1
+    S = alpha * xd + gd * hh * a
+    size = (alpha * xd).abs() + (gd * hh * a).abs() if g is not None \
+        else (alpha * xd).abs() + (hh * a).abs()
+    r2 = (S.square().mean(-1, keepdim=True) + eps).rsqrt()
+    sh = S * r2
+    within(s, S, u * S.abs() + slack * size + sub, "s")
+    within(n, sh * b, u * (sh * b).abs() + slack * size * r2 * b.abs() + sub,
+           "n")
+    dn, ds = dn.double(), ds.double()
+    dnw = dn * b
+    e = ds + r2 * (dnw - sh * (dnw * sh).mean(-1, keepdim=True))
+    big = size * r2
+    e_size = ds.abs() + r2 * (dnw.abs() + big * (dnw.abs() * big).mean(
+        -1, keepdim=True))
+    gg = gd.abs() if g is not None else 1.0
+    uu, u_size = gd * e * a, gg * e_size * a.abs()
+    want = [(r1 * (uu - hh * (uu * hh).mean(-1, keepdim=True)),
+             r1 * (u_size + hh.abs() * (u_size * hh.abs()).mean(
+                 -1, keepdim=True))),
+            (alpha * e, abs(alpha) * e_size)]
+    dims = tuple(range(len(shape) - 1))
+
+    def total(v, over):
+        return v.sum(over) if over else v
+
+    want.append((total(gd * e * hh, dims),
+                 total(gg * e_size * hh.abs(), dims)))
+    want.append((total(dn * sh, dims), total(dn.abs() * big, dims)))
+    if g is not None:
+        t, t_size = e * hh * a, e_size * (hh * a).abs()
+        keep = dims if g.dim() == 1 else \
+            dims[1:] if g.dim() == 2 and len(shape) > 2 else ()
+        want.append((total(t, keep), total(t_size, keep)))
+    for got, (w, m), name in zip(grads, want, ("dh", "dx", "dw1", "dw2",
+                                               "dg")):
+        within(got, w.view(got.shape), u * w.view(got.shape).abs()
+               + back * m.view(got.shape) + sub, name)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FP])
+@pytest.mark.parametrize("D", [1, 2, 7, 8, 64, 511, 512, 513, 1001, 1024,
+                               1032, 2048, 2056, 4096, 4100, 8192, 12001,
+                               16384])
+def test_block_norm_widths(D, dtype):
+    check_block_norm((3, 5, D), dtype, (3, D), 0.9, seed=D)
+
+
+@pytest.mark.parametrize("shape,gate", [
+    ((1, 64), None), ((1, 64), (64,)), ((1, 1, 520), (1, 520)),
+    ((7, 300, 96), None), ((7, 300, 96), (96,)), ((7, 300, 96), (7, 96)),
+    ((7, 300, 96), (7, 300, 96)), ((2100, 96), (2100, 96)),
+    ((5000, 3, 64), (5000, 64)),         # more gate rows than workers
+    ((4, 3, 5, 40), (4, 40)), ((6000, 1100), (1100,)), ((33,), (33,)),
+    ((2, 2500, 1500), (2, 1500)),
+])
+def test_block_norm_gates(shape, gate):
+    check_block_norm(shape, FP, gate, 1.25, seed=len(shape))
+    check_block_norm(shape, BF, gate, seed=len(shape))
+
+
+def test_block_norm_rows_of_zeros_and_scales():
+    D = 200
+    h = torch.zeros(4, D, device="cuda", dtype=BF)
+    w = torch.ones(D, device="cuda", dtype=BF)
+    n, s = fused_block_norm(h, h, w, w, None, 1.0, 1e-6)
+    assert (n == 0).all() and (s == 0).all()
+    check_block_norm((5, D), FP, (D,), 0.0, seed=1)      # no residual
+    check_block_norm((5, D), FP, (D,), -2.0, seed=2)
+    check_block_norm((5, D), FP, (D,), 1.0, 1e-2, seed=3)
+
+
+def test_block_norm_layouts_and_parts():
+    h, x = (normal((40, 6, 130), BF, i).transpose(0, 1) for i in (0, 1))
+    w = normal((260,), BF, 2)[::2]
+    a = fused_block_norm(h, x, w, w, w)
+    b = fused_block_norm(*(t.contiguous() for t in (h, x, w, w, w)))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    h.requires_grad_()
+    n, s = fused_block_norm(h, x, w, w)
+    (only_n,) = torch.autograd.grad(n, h, torch.ones_like(n),
+                                    retain_graph=True)
+    n2, s2 = fused_block_norm(h, x, w, w)
+    (both,) = torch.autograd.grad((n2, s2), h, (torch.ones_like(n),
+                                                torch.zeros_like(s)))
+    assert torch.equal(only_n, both)
+    e = fused_block_norm(h[:0], x[:0], w, w, w)
+    assert e[0].shape == (0, 40, 130)
+    z = torch.zeros(0, 8, device="cuda", requires_grad=True)
+    v = torch.ones(8, device="cuda", requires_grad=True)
+    n, s = fused_block_norm(z, z, v, v)
+    (dv,) = torch.autograd.grad(n.sum() + s.sum(), v)
+    assert (dv == 0).all()
+
+
+def test_block_norm_agrees_with_differences():
+    shape, D = (3, 4, 50), 50
+    t = [normal(shape, FP, 0), normal(shape, FP, 1),
+         normal((D,), FP, 2, 0.2, 1), normal((D,), FP, 3, 0.2, 1),
+         normal((3, D), FP, 4)]
+    dn, ds = normal(shape, FP, 5), normal(shape, FP, 6)
+    leaves = [x.requires_grad_() for x in t]
+    grads = torch.autograd.grad(fused_block_norm(*leaves), leaves, (dn, ds))
+
+    def forward(h, x, a, b, g):
+        z = h * (h.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * a
+        s = x + g[:, None] * z
+        n = s * (s.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * b
+        return (n * dn.double()).sum() + (s * ds.double()).sum()
+
+    base = [x.detach().double() for x in leaves]
+    for i, g in enumerate(grads):
+        d = normal(base[i].shape, torch.float64, 20 + i)
+        up, down = list(base), list(base)
+        up[i], down[i] = base[i] + 1e-4 * d, base[i] - 1e-4 * d
+        slope = (forward(*up) - forward(*down)) / 2e-4
+        along = (g.double() * d).sum()
+        # 2^-15 of the terms' sizes, at most a few for each element
+        assert (slope - along).abs() <= 2.0 ** -15 * 40 * d.abs().sum() + 1e-4
+
+
+# ---- clipping --------------------------------------------------------------
+
+def params_of(specs, seed=0, scale=1.0):
+    out = []
+    for i, (shape, dtype) in enumerate(specs):
+        p = torch.nn.Parameter(torch.empty(shape, device="cuda", dtype=dtype))
+        p.grad = normal(shape, dtype, seed + i, scale)
+        out.append(p)
+    return out
+
+
+def check_clip(params, max_norm):
+    before = [p.grad.double() for p in params]
+    total = sum(g.square().sum() for g in before) ** 0.5
+    n0 = grad_norm(params)
+    n1 = clip_grad_norm_(params, max_norm)
+    for n in (n0, n1):
+        assert n.dtype == FP and n.dim() == 0
+        assert (n.double() - total).abs() <= 2.0 ** -23 * total
+    c = min(1.0, max_norm / (float(total) + 1e-6))
+    for p, g in zip(params, before):
+        if c == 1.0:
+            assert torch.equal(p.grad.double(), g)
+            continue
+        w = g * c   # the factor, the product and the result are rounded
+        within(p.grad, w, (unit(p.dtype) + 2 * 2.0 ** -24) * w.abs()
+               + subnormal(p.dtype) + 2.0 ** -134, "clipped")
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 0.5, 1e9])
+@pytest.mark.parametrize("specs", [
+    [((1,), FP)], [((7, 3), BF), ((1,), FH), ((8193,), FP)],
+    [((8192,), BF), ((8191,), BF), ((3, 5, 7), FH), ((0,), FP)],
+    [((i % 23 + 1,), (BF, FH, FP)[i % 3]) for i in range(500)],
+    [((1000, 1001), BF), ((333,), FP), ((4097, 513), FH)],
+])
+def test_clip(specs, max_norm):
+    check_clip(params_of(specs), max_norm)
+
+
+def test_clip_views_of_one_bucket():
+    """Gradients that begin anywhere in a flat bucket: what lies between
+    them stays as it was."""
+    for dtype in (BF, FH, FP):
+        flat = normal((40_000,), dtype, 3)
+        keep, params, at = flat.clone(), [], 1
+        used = torch.zeros(40_000, dtype=torch.bool, device="cuda")
+        for n in (1, 3, 8, 9, 15, 100, 8191, 20_001):
+            p = torch.nn.Parameter(torch.empty(n, device="cuda", dtype=dtype))
+            p.grad = flat[at:at + n]
+            used[at:at + n] = True
+            at += n + 1
+            params.append(p)
+        check_clip(params, 0.25)
+        assert torch.equal(flat[~used], keep[~used])
+
+
+def test_clip_range():
+    """Squares outside the range of fp32, sums of tiny and huge values."""
+    for scale in (1e-30, 1e-20, 1e18, 1e30):
+        p = params_of([((5000,), FP), ((300,), BF)], 1, scale)
+        check_clip(p, scale)
+    p = params_of([((4096,), FP)], 2)
+    p[0].grad[17] = math.inf
+    assert clip_grad_norm_(p, 1.0).isinf()
+    g = p[0].grad
+    assert g[17].isnan() and (g[:17] == 0).all() and (g[18:] == 0).all()
+    p = params_of([((4096,), BF), ((9,), FP)], 2)
+    p[0].grad[17] = math.nan
+    assert clip_grad_norm_(p, 1.0).isnan()
+    assert all(x.grad.isnan().all() for x in p)
+
+
+def test_clip_layouts_and_ties():
+    p = params_of([((16, 8, 3, 3), BF), ((64, 32), FP)])
+    p[0].grad = p[0].grad.contiguous(memory_format=torch.channels_last)
+    p[1].grad = p[1].grad.t().contiguous().t()
+    check_clip(p, 0.5)
+    q = params_of([((50,), FP)])
+    before = q[0].grad.double()
+    n = clip_grad_norm_([q[0], q[0]], 1.0)     # a tied weight counts once
+    assert (n.double() - before.norm()).abs() <= 2.0 ** -23 * before.norm()
+    q.append(torch.nn.Parameter(torch.empty(3, device="cuda")))
+    clip_grad_norm_(q, 1.0)                    # one without a gradient
+    assert q[1].grad is None
+    assert grad_norm(q[1:]) == 0
+    v = q[0].grad._version
+    clip_grad_norm_(q, 1.0)
+    assert q[0].grad._version > v
+
+
+def test_clip_long_tensor():
+    """More than 2^31 values: offsets pass 32 bits."""
+    n = (1 << 31) + 12345
+    p = torch.nn.Parameter(torch.empty(0, device="cuda", dtype=BF))
+    p.data = torch.empty(n, device="cuda", dtype=BF)
+    p.grad = torch.zeros(n, device="cuda", dtype=BF)
+    p.grad[0] = p.grad[-1] = p.grad[1 << 30] = p.grad[(1 << 31) + 5] = 1.0
+    assert clip_grad_norm_([p], 1.0) == 2.0
+    at = [i * (1 << 30) + int(j) for i, part in
+          enumerate(p.grad.split(1 << 30)) for j in part.nonzero()]
+    assert at == [0, 1 << 30, (1 << 31) + 5, n - 1]
+    assert (p.grad[at] == 0.5).all()
+
+
+# ---- streams, graphs, refusals on the device -------------------------------
+
+def step_of(state):
+    """One block's step over packed tokens, as a user would run it."""
+    h0, weights, cu, pos, cos, sin, norm, params = state
+    wqkv, wo = weights
+    T, hidden = h0.shape
+    H, HK, D = 4, 2, 64
+    qkv = h0 @ wqkv
+    q, k, v = qkv.split([H * D, HK * D, HK * D], -1)
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in (q, k, v))
+    q, k = fused_rope_axes(q, k, pos, cos, sin, [8, 12, 12])
+    o = flash_attention_packed(q, k, v, cu, causal=True)
+    n, s = norm(o.reshape(T, H * D) @ wo, h0)
+    loss = (n.float().square().mean() + s.float().mean())
+    grads = torch.autograd.grad(loss, params)
+    for p, g in zip(params, grads):
+        p.grad.copy_(g)
+    total = clip_grad_norm_(params, 0.01)
+    return loss.detach(), total
+
+
+def make_state(seed=0, T=300):
+    hidden, H, HK, D = 256, 4, 2, 64
+    h0 = normal((T, hidden), BF, seed)
+    ws = [torch.nn.Parameter(normal(s, BF, seed + i, 0.06)) for i, s in
+          enumerate([(hidden, (H + 2 * HK) * D), (H * D, hidden)], 1)]
+    norm = FusedBlockNorm(hidden, residual_scale=0.9, gated=True,
+                          gate_init=0.3).to(device="cuda", dtype=BF)
+    params = ws + list(norm.parameters())
+    for p in params:
+        p.grad = torch.zeros_like(p)
+    cos, sin = rope_tables(400, 32)
+    pos = torch.randint(0, 400, (3, T), device="cuda")
+    return h0, ws, cu_of([120, 0, 150]), pos, cos, sin, norm, params
+
+
+def test_together_against_64_bits():
+    """The four as one step; the oracle runs the same in 64 bits.  Each
+    stage rounds its outputs and the products theirs: ten roundings of
+    relative size 2^-9 between the loss and a weight's gradient, whose
+    errors do not line up; 5% of a gradient's norm is over ten times
+    sqrt(10) of them."""
+    state = make_state()
+    h0, (wqkv, wo), cu, pos, cos, sin, norm, params = state
+    loss, total = step_of(state)
+    ps = [p.detach().double().requires_grad_() for p in params]
+    T, D = h0.shape[0], 64
+    x = h0.double()
+    q, k, v = (x @ ps[0]).split([256, 128, 128], -1)
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in (q, k, v))
+    axis = [0] * 8 + [1] * 12 + [2] * 12
+    at = pos[axis].t()
+    j = torch.arange(32, device="cuda")
+    c, s = (t[at, j].double()[:, None] for t in (cos, sin))
+    q, k = (torch.cat([t[..., :32] * c - t[..., 32:] * s,
+                       t[..., 32:] * c + t[..., :32] * s], -1)
+            for t in (q, k))
+    seen = seen_of([120, 0, 150], None, T, True, None)
+    k, v = (t.repeat_interleave(2, 1) for t in (k, v))
+    z = (q.transpose(0, 1) @ k.permute(1, 2, 0)) / 8
+    z = z.masked_fill(~seen, -math.inf).masked_fill(
+        ~seen.any(1)[:, None], 0.0)
+    p = torch.softmax(z, -1) * seen.any(1)[:, None]
+    o = (p @ v.transpose(0, 1)).transpose(0, 1).reshape(T, 256) @ ps[1]
+    w1, w2, g = (dict(norm.named_parameters())[n] for n in
+                 ("post_weight", "pre_weight", "gate"))
+    index = {id(a): b for a, b in zip(params, ps)}
+    w1, w2, g = (index[id(t)] for t in (w1, w2, g))
+    S = 0.9 * x + g * o * (o.square().mean(-1, keepdim=True)
+                           + 1e-6).rsqrt() * w1
+    N = S * (S.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w2
+    want = N.square().mean() + S.mean()
+    grads = torch.autograd.grad(want, ps)
+    norm_all = sum(t.square().sum() for t in grads) ** 0.5
+    assert (loss.double() - want).abs() <= 2.0 ** -8 * want.abs()
+    assert (total.double() - norm_all).abs() <= 0.05 * norm_all
+    c = min(1.0, 0.01 / float(norm_all))
+    for p, t in zip(params, grads):
+        assert (p.grad.double() - c * t).norm() <= 0.05 * c * norm_all
+    opt = FusedAdamW(params, lr=1e-3)
+    opt.step()                       # what stands behind it still runs
+    assert all(torch.isfinite(p).all() for p in params)
+
+
+def test_together_captured_and_replayed():
+    state = make_state(5)
+    params = state[-1]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step_of(state)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, total = step_of(state)
+    for i in range(4):
+        h = normal(state[0].shape, BF, 100 + i)
+        cu = [[120, 0, 150], [1, 2, 3], [300, 0, 0], [0, 0, 0]][i]
+        state[0].copy_(h)
+        state[2].copy_(cu_of(cu))
+        want_loss, want_total = step_of(state)
+        want = [p.grad.clone() for p in params]
+        for p in params:
+            p.grad.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want_loss) and torch.equal(total, want_total)
+        assert all(torch.equal(p.grad, w) for p, w in zip(params, want))
+
+
+def test_together_on_two_streams():
+    """Two steps at once on streams of their own share nothing."""
+    states = [make_state(s) for s in (11, 12)]
+    want = []
+    for st in states:
+        out = step_of(st)
+        want.append([t.clone() for t in out] + [p.grad.clone()
+                                                for p in st[-1]])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    for _ in range(5):
+        got = []
+        for st, stream in zip(states, streams):
+            with torch.cuda.stream(stream):
+                got.append(step_of(st))
+        torch.cuda.synchronize()
+        for st, g, w in zip(states, got, want):
+            now = list(g) + [p.grad for p in st[-1]]
+            assert all(torch.equal(a, b) for a, b in zip(now, w))
+
+
+def test_refusals_on_the_device():
+    q = torch.zeros(8, 2, 64, device="cuda", dtype=BF)
+    cu = cu_of([8])
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        flash_attention_packed(q.float(), q.float(), q.float(), cu)
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        flash_attention_packed(q, q.half(), q.half(), cu)
+    with pytest.raises(ValueError, match="one device"):
+        flash_attention_packed(q, q, q, cu.cpu())
+    cos, sin = rope_tables(8, 32)
+    pos = torch.zeros(1, 8, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="one device"):
+        fused_rope_axes(q, q, pos, cos.cpu(), sin.cpu(), [32])
+    w = torch.ones(64, device="cuda", dtype=BF)
+    with pytest.raises(ValueError, match="type and device"):
+        fused_block_norm(q, q, w.float(), w)
+    p = params_of([((8,), FP), ((8,), FP)])
+    flat = torch.zeros(12, device="cuda")
+    p[0].grad, p[1].grad = flat[:8], flat[4:]
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_(p, 1.0)
+    p[1].grad = torch.zeros(1, device="cuda").expand(8)
+    with pytest.raises(RuntimeError, match="dense"):
+        clip_grad_norm_(p, 1.0)
+    d = torch.nn.Parameter(torch.zeros(3, device="cuda",
+                                       dtype=torch.float64))
+    d.grad = torch.zeros_like(d)
+    with pytest.raises(RuntimeError, match="bf16, fp16 or fp32"):
+        clip_grad_norm_([d], 1.0)
+    # a second derivative is refused, not wrong
+    x = torch.ones(2, 8, device="cuda", requires_grad=True)
+    v = torch.ones(8, device="cuda", requires_grad=True)
+    n, _ = fused_block_norm(x, x, v, v)
+    (g,) = torch.autograd.grad(n.sum(), v, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
