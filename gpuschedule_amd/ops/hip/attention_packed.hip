@@ -84,9 +84,10 @@ struct Args {
   const short *q, *k, *v, *o, *dout;
   short *out, *dq, *dk, *dv;
   float *lse, *drow;               // [H, T]; lse in units of log 2
+  float* part;                     // [splits][dk, dv][T, HK, D]
   const int *cu, *lengths;         // lengths may be null
   long q_t, q_h, k_t, k_h, v_t, v_h, d_t, d_h;  // strides; d: dout
-  int T, B, H, HK, D, units, window;            // window 0: none
+  int T, B, H, HK, D, slots, splits, window;    // window 0: none
   float scale;
 };
 
@@ -119,19 +120,22 @@ __device__ __forceinline__ bool tile_of(const Args& a, int slot, Seq& s,
   return row0 >= 0 && row0 < s.rows;
 }
 
-// A unit is one kv head's share of one slot; its `rep` query heads are
+// A unit is one slot of one of `heads` kv heads; its `rep` query heads are
 // neighbours in time on one XCD (blocks go to the 8 XCDs in turn), so that
-// they find its keys in that XCD's L2.  kv heads change fastest, so that
-// every XCD gets tiles of all places; late slots, the long ones under a
-// causal mask, go first.
-__device__ __forceinline__ bool unit_of(const Args& a, int rep, int& kvh,
-                                        int& slot, int& sub) {
+// they find its keys in that XCD's L2.  Heads change fastest, so that every
+// XCD gets tiles of all places; `late` slots go first where those are the
+// long ones.
+__device__ __forceinline__ bool unit_of(const Args& a, int heads, int rep,
+                                        bool late, int& head, int& slot,
+                                        int& sub) {
   const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
   const int unit = j / rep * 8 + xcd;
   sub = j % rep;
-  kvh = unit % a.HK;
-  slot = a.units / a.HK - 1 - unit / a.HK;
-  return unit < a.units;
+  head = unit % heads;
+  slot = unit / heads;
+  if (slot >= a.slots) return false;
+  if (late) slot = a.slots - 1 - slot;
+  return true;
 }
 
 // ---- LDS tiles ---------------------------------------------------------
@@ -145,25 +149,44 @@ template <int DP> __device__ __forceinline__ int mix(int r) {
   return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
 }
 
-// Rows row0.. of p (row stride `ld`) to LDS without passing registers.
+// Rows of p (stride `ld`) go to LDS without passing registers, 16 bytes a
+// lane.  One offset a lane serves all of its pieces: they are NTH / NCH rows
+// apart, at which the swizzle repeats, so the rest of the address is uniform.
+template <int DP>
+__device__ __forceinline__ unsigned stage_offset(long ld) {
+  constexpr int NCH = DP / 8;
+  const int r = threadIdx.x / NCH, c = (threadIdx.x % NCH) ^ mix<DP>(r);
+  return (unsigned)(r * ld * 2 + c * 16);
+}
+
+__device__ __forceinline__ void to_lds(const void* src, char* tile, int it) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) unsigned*)src,
+      (__attribute__((address_space(3))) unsigned*)
+          (tile + (it * NTH + (threadIdx.x & ~63)) * 16),
+      16, 0, 0);
+}
+
 // Rows from `rows` on and values from D on are zeros: those lanes read
 // zeros instead, so nothing of another sequence ever enters a product.
-template <int DP>
-__device__ __forceinline__ void stage(const short* p, long ld, int row0,
-                                      int rows, int D, char* tile) {
-  constexpr int NCH = DP / 8;
+template <int DP, int ROWS>
+__device__ __forceinline__ void stage(const short* p, long ld, unsigned off,
+                                      int row0, int rows, int D, char* tile) {
+  constexpr int NCH = DP / 8, STEP = NTH / NCH;
+  if (row0 + ROWS <= rows && D == DP) {
+    const char* g = (const char*)(p + row0 * ld);
 #pragma unroll
-  for (int it = 0; it < TILE * NCH / NTH; ++it) {
-    const int at = it * NTH + threadIdx.x;
-    const int r = at / NCH, c = (at % NCH) ^ mix<DP>(r);
-    const bool ok = row0 + r < rows && c * 8 < D;
-    const short* g = p + (long)(row0 + r) * ld + c * 8;
-    const void* src = ok ? (const void*)g : (const void*)&kZeros;
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) unsigned*)src,
-        (__attribute__((address_space(3))) unsigned*)
-            (tile + (it * NTH + (threadIdx.x & ~63)) * 16),
-        16, 0, 0);
+    for (int it = 0; it < ROWS / STEP; ++it)
+      to_lds(g + it * (STEP * ld * 2) + off, tile, it);
+  } else {
+#pragma unroll
+    for (int it = 0; it < ROWS / STEP; ++it) {
+      const int r = it * STEP + threadIdx.x / NCH;
+      const int c = (threadIdx.x % NCH) ^ mix<DP>(r);
+      const bool ok = row0 + r < rows && c * 8 < D;
+      const short* g = p + (row0 + r) * ld + c * 8;
+      to_lds(ok ? (const void*)g : (const void*)&kZeros, tile, it);
+    }
   }
 }
 
@@ -227,27 +250,60 @@ __device__ __forceinline__ void put_rows(short* p, bool live, int D, int lane,
 
 // The other half's value (lane l ^ 32).
 __device__ __forceinline__ float other_half(float v) {
-  return __shfl_xor(v, 32, WAVE);
+  const auto r = __builtin_amdgcn_permlane32_swap(
+      __builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false,
+      false);
+  // r[0]: the low half's value in both halves, r[1]: the high half's
+  return __builtin_bit_cast(float, threadIdx.x & 32 ? r[0] : r[1]);
+}
+
+// 2^x; results under 2^-126 are 0
+__device__ __forceinline__ float exp2_of(float x) {
+  return __builtin_amdgcn_exp2f(x);
 }
 
 constexpr float kNone = -INFINITY;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// What the rows first..first + 31 of a wave see of the tile at kv0: nothing
+// (0), part of it (1) or all of it (2).
+template <bool CAUSAL>
+__device__ __forceinline__ int sees(const Args& a, int kv0, int first,
+                                    int len) {
+  const int last = first + 31;
+  if (first >= len || (CAUSAL && kv0 > last) ||
+      (a.window && kv0 + TILE <= first - a.window + 1))
+    return 0;
+  return kv0 + TILE > len || (CAUSAL && kv0 + TILE - 1 > first) ||
+                 (a.window && kv0 <= last - a.window)
+             ? 1 : 2;
+}
+
+template <bool CAUSAL>
+__device__ __forceinline__ bool seen(const Args& a, int key, int row,
+                                     int len) {
+  return key < len && (!CAUSAL || key <= row) &&
+         (!a.window || key > row - a.window);
+}
 
 // ---- forward -----------------------------------------------------------
 
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.H / a.HK;
   int kvh, slot, sub, row0;
   Seq s;
-  if (!unit_of(a, rep, kvh, slot, sub)) return;
+  if (!unit_of(a, a.HK, rep, CAUSAL, kvh, slot, sub)) return;
   if (!tile_of<OWN>(a, slot, s, row0)) return;
   const int head = kvh * rep + sub;
-  const int row = row0 + wave * 32 + (lane & 31);
+  const int first = row0 + wave * 32, row = first + (lane & 31);
   const bool live = row < s.len;
   const long at = s.begin + row;
 
+  // m: the reference that exponents are taken from, in units of log 2
   float m = kNone, l = 0.f;
   float16v o[DP / 32];
 #pragma unroll
@@ -256,27 +312,28 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
   if (row0 < s.len) {
     short8 q[DP / 16];
     own_rows<DP>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
-    const short* kp = a.k + (long)s.begin * a.k_t + kvh * a.k_h;
-    const short* vp = a.v + (long)s.begin * a.v_t + kvh * a.v_h;
+    const short* kp = a.k + s.begin * a.k_t + kvh * a.k_h;
+    const short* vp = a.v + s.begin * a.v_t + kvh * a.v_h;
+    const unsigned koff = stage_offset<DP>(a.k_t);
+    const unsigned voff = stage_offset<DP>(a.v_t);
     const int end = CAUSAL ? min(s.len, row0 + OWN) : s.len;
-    int t0 = 0;
-    if (a.window) t0 = max(row0 - a.window + 1, 0) / TILE;
+    const int t0 = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
     const int t1 = (end + TILE - 1) / TILE;
-    const int first = row0 + wave * 32, last = first + 31;
-    const float sl2 = a.scale * 1.44269504088896340736f;
-    stage<DP>(kp, a.k_t, t0 * TILE, s.len, a.D, lds[0]);
-    stage<DP>(vp, a.v_t, t0 * TILE, s.len, a.D, lds[1]);
+    const float sl2 = a.scale * kLog2e;
+    stage<DP, TILE>(kp, a.k_t, koff, t0 * TILE, s.len, a.D, lds[0]);
+    stage<DP, TILE>(vp, a.v_t, voff, t0 * TILE, s.len, a.D, lds[1]);
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
+    int buf = 0;
+    for (int t = t0; t < t1; ++t, buf ^= 2) {
       const int kv0 = t * TILE;
-      char* kt = lds[(t - t0) & 1 ? 2 : 0];
-      char* vt = lds[(t - t0) & 1 ? 3 : 1];
+      const char *kt = lds[buf], *vt = lds[buf + 1];
       if (t + 1 < t1) {
-        stage<DP>(kp, a.k_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 0 : 2]);
-        stage<DP>(vp, a.v_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 1 : 3]);
+        stage<DP, TILE>(kp, a.k_t, koff, kv0 + TILE, s.len, a.D, lds[buf ^ 2]);
+        stage<DP, TILE>(vp, a.v_t, voff, kv0 + TILE, s.len, a.D,
+                        lds[(buf ^ 2) + 1]);
       }
-      if ((!CAUSAL || kv0 <= last) && first < s.len &&
-          (!a.window || kv0 + TILE > first - a.window + 1)) {
+      const int what = sees<CAUSAL>(a, kv0, first, s.len);
+      if (what) {
         float16v sc[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -285,20 +342,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           for (int kk = 0; kk < DP / 16; ++kk)
             sc[kb] = E::mfma(rows_of<DP>(kt, 32 * kb, kk, lane), q[kk], sc[kb]);
         }
-        const bool edge = kv0 + TILE > s.len ||
-                          (CAUSAL && kv0 + TILE - 1 > first) ||
-                          (a.window && kv0 <= last - a.window);
-        if (edge) {
+        if (what == 1) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int key = kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) +
-                              i % 4;
-              bool seen = key < s.len;
-              if (CAUSAL) seen &= key <= row;
-              if (a.window) seen &= key > row - a.window;
-              if (!seen) sc[kb][i] = kNone;
+              const int key =
+                  kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+              if (!seen<CAUSAL>(a, key, row, s.len)) sc[kb][i] = kNone;
             }
         }
         float top = kNone;
@@ -307,21 +358,26 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
         top = fmaxf(top, other_half(top)) * sl2;
-        const float mn = fmaxf(m, top);
-        const float ref = mn == kNone ? 0.f : mn;
-        const float alpha = exp2f(m - ref);
-        m = mn;
-        l *= alpha;
+        // The reference moves only where a maximum leaves it by more than
+        // 2^8: o and l are fp32, and probabilities keep their relative
+        // precision up to there, in fp16 too.
+        if (__any(top > m + 8.f)) {
+          const float mn = fmaxf(m, top);
+          const float alpha = mn == kNone ? 0.f : exp2_of(m - mn);
+          m = mn;
+          l *= alpha;
 #pragma unroll
-        for (int f = 0; f < DP / 32; ++f)
+          for (int f = 0; f < DP / 32; ++f)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[f][i] *= alpha;
+            for (int i = 0; i < 16; ++i) o[f][i] *= alpha;
+        }
+        const float ref = m == kNone ? 0.f : m;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           float p[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            p[j] = exp2f(sc[ks / 2][8 * (ks & 1) + j] * sl2 - ref);
+            p[j] = exp2_of(sc[ks / 2][8 * (ks & 1) + j] * sl2 - ref);
             l += p[j];
           }
           // probabilities are rounded to the type of v, which the matrix
@@ -350,14 +406,15 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.H / a.HK;
   int kvh, slot, sub, row0;
   Seq s;
-  if (!unit_of(a, rep, kvh, slot, sub)) return;
+  if (!unit_of(a, a.HK, rep, CAUSAL, kvh, slot, sub)) return;
   if (!tile_of<OWN>(a, slot, s, row0)) return;
   const int head = kvh * rep + sub;
-  const int row = row0 + wave * 32 + (lane & 31);
+  const int first = row0 + wave * 32, row = first + (lane & 31);
   const bool live = row < s.len;
   const long at = s.begin + row;
 
@@ -382,30 +439,28 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     }
     const float lse = live ? a.lse[(long)head * a.T + at] : INFINITY;
     if (live && lane < 32) a.drow[(long)head * a.T + at] = dr;
-    const short* kp = a.k + (long)s.begin * a.k_t + kvh * a.k_h;
-    const short* vp = a.v + (long)s.begin * a.v_t + kvh * a.v_h;
+    const short* kp = a.k + s.begin * a.k_t + kvh * a.k_h;
+    const short* vp = a.v + s.begin * a.v_t + kvh * a.v_h;
+    const unsigned koff = stage_offset<DP>(a.k_t);
+    const unsigned voff = stage_offset<DP>(a.v_t);
     const int end = CAUSAL ? min(s.len, row0 + OWN) : s.len;
-    int t0 = 0;
-    if (a.window) t0 = max(row0 - a.window + 1, 0) / TILE;
+    const int t0 = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
     const int t1 = (end + TILE - 1) / TILE;
-    const int first = row0 + wave * 32, last = first + 31;
-    const float sl2 = a.scale * 1.44269504088896340736f;
-    stage<DP>(kp, a.k_t, t0 * TILE, s.len, a.D, lds[0]);
-    stage<DP>(vp, a.v_t, t0 * TILE, s.len, a.D, lds[1]);
+    const float sl2 = a.scale * kLog2e;
+    stage<DP, TILE>(kp, a.k_t, koff, t0 * TILE, s.len, a.D, lds[0]);
+    stage<DP, TILE>(vp, a.v_t, voff, t0 * TILE, s.len, a.D, lds[1]);
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
+    int buf = 0;
+    for (int t = t0; t < t1; ++t, buf ^= 2) {
       const int kv0 = t * TILE;
-      char* kt = lds[(t - t0) & 1 ? 2 : 0];
-      char* vt = lds[(t - t0) & 1 ? 3 : 1];
+      const char *kt = lds[buf], *vt = lds[buf + 1];
       if (t + 1 < t1) {
-        stage<DP>(kp, a.k_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 0 : 2]);
-        stage<DP>(vp, a.v_t, kv0 + TILE, s.len, a.D, lds[(t - t0) & 1 ? 1 : 3]);
+        stage<DP, TILE>(kp, a.k_t, koff, kv0 + TILE, s.len, a.D, lds[buf ^ 2]);
+        stage<DP, TILE>(vp, a.v_t, voff, kv0 + TILE, s.len, a.D,
+                        lds[(buf ^ 2) + 1]);
       }
-      if ((!CAUSAL || kv0 <= last) && first < s.len &&
-          (!a.window || kv0 + TILE > first - a.window + 1)) {
-        const bool edge = kv0 + TILE > s.len ||
-                          (CAUSAL && kv0 + TILE - 1 > first) ||
-                          (a.window && kv0 <= last - a.window);
+      const int what = sees<CAUSAL>(a, kv0, first, s.len);
+      if (what) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
           float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
@@ -414,21 +469,19 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
             sc = E::mfma(rows_of<DP>(kt, 32 * kb, kk, lane), q[kk], sc);
             dp = E::mfma(rows_of<DP>(vt, 32 * kb, kk, lane), dO[kk], dp);
           }
-          float ds[16];
+          if (what == 1) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float p = exp2f(sc[i] * sl2 - lse);
-            if (edge) {
-              const int key = kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) +
-                              i % 4;
-              bool seen = key < s.len;
-              if (CAUSAL) seen &= key <= row;
-              if (a.window) seen &= key > row - a.window;
-              if (!seen) p = 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const int key =
+                  kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+              if (!seen<CAUSAL>(a, key, row, s.len)) sc[i] = kNone;
             }
-            // dS is rounded to the type of k, which the product needs
-            ds[i] = p * (dp[i] * a.scale - dr);
           }
+          float ds[16];
+          // dS is rounded to the type of k, which the product needs
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            ds[i] = exp2_of(sc[i] * sl2 - lse) * (dp[i] * a.scale - dr);
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             const short8 b = E::pack(ds + 8 * ks);
@@ -448,19 +501,31 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 
 // ---- backward: dK and dV -----------------------------------------------
 // A block owns 128 keys of one kv head and goes through the query tiles of
-// all its heads: shared heads add up in registers, in a fixed order.
+// `rep / splits` of its heads.  Where kv heads and tiles are too few to fill
+// the card, the heads are split among blocks, which leave their sums in
+// fp32, and one more kernel adds those in a fixed order.
+//
+// Registers are what this kernel is short of: two accumulators of 32 x DP
+// and a fragment of k take 160 of the 256 that two waves on a SIMD leave, so
+// v stays in LDS, and query tiles are 32 rows.
+
+constexpr int QT = 32;
 
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(NTH, 1) void packed_bwd_kv_kernel(const Args a) {
-  __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][TILE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rep = a.H / a.HK;
-  int kvh, slot, sub, row0;
+__global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char own_v[OWN * DP * 2];
+  __shared__ __attribute__((aligned(16))) char lds[4][QT * DP * 2];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][QT];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rep = a.H / a.HK, mine = rep / a.splits;
+  int vh, slot, none, row0;
   Seq s;
-  if (!unit_of(a, 1, kvh, slot, sub)) return;
+  if (!unit_of(a, a.HK * a.splits, 1, false, vh, slot, none)) return;
   if (!tile_of<OWN>(a, slot, s, row0)) return;
-  const int key = row0 + wave * 32 + (lane & 31);
+  const int kvh = vh / a.splits, split = vh % a.splits;
+  const int h0 = kvh * rep + split * mine;
+  const int first = row0 + wave * 32, key = first + (lane & 31);
   const bool live = key < s.len;
   const long at = s.begin + key;
 
@@ -469,80 +534,127 @@ __global__ __launch_bounds__(NTH, 1) void packed_bwd_kv_kernel(const Args a) {
   for (int f = 0; f < DP / 32; ++f) dk[f] = dv[f] = (float16v)(0.f);
 
   if (row0 < s.len) {
-    short8 k[DP / 16], v[DP / 16];
+    short8 k[DP / 16];
     own_rows<DP>(a.k + at * a.k_t + kvh * a.k_h, live, a.D, lane, k);
-    own_rows<DP>(a.v + at * a.v_t + kvh * a.v_h, live, a.D, lane, v);
-    const int t0 = CAUSAL ? row0 / TILE : 0;
+    stage<DP, OWN>(a.v + s.begin * a.v_t + kvh * a.v_h, a.v_t,
+                   stage_offset<DP>(a.v_t), row0, s.len, a.D, own_v);
+    const unsigned qoff = stage_offset<DP>(a.q_t);
+    const unsigned doff = stage_offset<DP>(a.d_t);
+    const int t0 = CAUSAL ? row0 / QT : 0;
     int end = s.len;
-    if (a.window) end = min((long)end, (long)row0 + OWN - 1 + a.window);
-    const int tiles = (end + TILE - 1) / TILE - t0;
-    const int first = row0 + wave * 32, last = first + 31;
-    const float sl2 = a.scale * 1.44269504088896340736f;
-    auto fetch = [&](int n, int buf) {
-      const int head = kvh * rep + n / tiles, q0 = (t0 + n % tiles) * TILE;
-      stage<DP>(a.q + (long)s.begin * a.q_t + head * a.q_h, a.q_t, q0, s.len,
-                a.D, lds[2 * buf]);
-      stage<DP>(a.dout + (long)s.begin * a.d_t + head * a.d_h, a.d_t, q0,
-                s.len, a.D, lds[2 * buf + 1]);
-      if (threadIdx.x < TILE) {
-        const int row = q0 + threadIdx.x;
+    if (a.window) end = min(end, row0 + OWN - 1 + a.window);
+    const int t1 = (end + QT - 1) / QT;
+    const int last = first + 31;
+    const float sl2 = a.scale * kLog2e;
+    auto fetch = [&](int head, int t, int buf) {
+      stage<DP, QT>(a.q + s.begin * a.q_t + head * a.q_h, a.q_t, qoff, t * QT,
+                    s.len, a.D, lds[2 * buf]);
+      stage<DP, QT>(a.dout + s.begin * a.d_t + head * a.d_h, a.d_t, doff,
+                    t * QT, s.len, a.D, lds[2 * buf + 1]);
+      if (threadIdx.x < QT) {
+        const int row = t * QT + threadIdx.x;
         const long e = (long)head * a.T + s.begin + row;
         const bool ok = row < s.len;
         stat[buf][0][threadIdx.x] = ok ? a.lse[e] : INFINITY;
         stat[buf][1][threadIdx.x] = ok ? a.drow[e] : 0.f;
       }
     };
-    fetch(0, 0);
+    fetch(h0, t0, 0);
     __syncthreads();
-    for (int n = 0; n < rep * tiles; ++n) {
-      const int buf = n & 1, q0 = (t0 + n % tiles) * TILE;
-      if (n + 1 < rep * tiles) fetch(n + 1, buf ^ 1);
-      const char *qt = lds[2 * buf], *dt = lds[2 * buf + 1];
-      if ((!CAUSAL || q0 + TILE > first) && first < s.len &&
-          (!a.window || q0 <= last + a.window - 1)) {
-        const bool edge = (CAUSAL && q0 < last) ||
-                          (a.window && q0 + TILE - 1 >= first + a.window);
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
+    int buf = 0;
+    for (int head = h0; head < h0 + mine; ++head)
+      for (int t = t0; t < t1; ++t, buf ^= 1) {
+        const int q0 = t * QT;
+        if (t + 1 < t1) fetch(head, t + 1, buf ^ 1);
+        else if (head + 1 < h0 + mine) fetch(head + 1, t0, buf ^ 1);
+        const char *qt = lds[2 * buf], *dt = lds[2 * buf + 1];
+        if ((!CAUSAL || q0 + QT > first) && first < s.len &&
+            (!a.window || q0 <= last + a.window - 1)) {
           float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
-            sc = E::mfma(rows_of<DP>(qt, 32 * qb, kk, lane), k[kk], sc);
-            dp = E::mfma(rows_of<DP>(dt, 32 * qb, kk, lane), v[kk], dp);
+            sc = E::mfma(rows_of<DP>(qt, 0, kk, lane), k[kk], sc);
+            dp = E::mfma(rows_of<DP>(dt, 0, kk, lane),
+                         rows_of<DP>(own_v, wave * 32, kk, lane), dp);
+          }
+          if ((CAUSAL && q0 < last) ||
+              (a.window && q0 + QT - 1 >= first + a.window)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int row = q0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+              if (!seen<CAUSAL>(a, key, row, s.len)) sc[i] = kNone;
+            }
           }
           float p[16], ds[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = 32 * qb + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-            p[i] = exp2f(sc[i] * sl2 - stat[buf][0][r]);
-            if (edge) {
-              bool seen = true;
-              if (CAUSAL) seen &= key <= q0 + r;
-              if (a.window) seen &= key > q0 + r - a.window;
-              if (!seen) p[i] = 0.f;
+          for (int g = 0; g < 4; ++g) {
+            const int r = 8 * g + 4 * (lane >> 5);
+            const float4v ls = *reinterpret_cast<float4v*>(&stat[buf][0][r]);
+            const float4v dr = *reinterpret_cast<float4v*>(&stat[buf][1][r]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int i = 4 * g + j;
+              p[i] = exp2_of(sc[i] * sl2 - ls[j]);
+              ds[i] = p[i] * (dp[i] * a.scale - dr[j]);
             }
-            ds[i] = p[i] * (dp[i] * a.scale - stat[buf][1][r]);
           }
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             const short8 pb = E::pack(p + 8 * ks), sb = E::pack(ds + 8 * ks);
 #pragma unroll
             for (int f = 0; f < DP / 32; ++f) {
-              dv[f] = E::mfma(cols_of<DP>(dt, 32 * qb + 16 * ks, f, lane), pb,
-                              dv[f]);
-              dk[f] = E::mfma(cols_of<DP>(qt, 32 * qb + 16 * ks, f, lane), sb,
-                              dk[f]);
+              dv[f] = E::mfma(cols_of<DP>(dt, 16 * ks, f, lane), pb, dv[f]);
+              dk[f] = E::mfma(cols_of<DP>(qt, 16 * ks, f, lane), sb, dk[f]);
             }
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
-    }
   }
-  if (key < s.rows) {
+  if (key >= s.rows) return;
+  if (a.splits == 1) {
     put_rows<E, DP>(a.dk + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dk);
     put_rows<E, DP>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dv);
+  } else {
+    const long n = (long)a.T * a.HK * a.D;
+    float* p = a.part + (2 * split * a.T + at) * a.HK * a.D + kvh * a.D;
+#pragma unroll
+    for (int f = 0; f < DP / 32; ++f)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * f + 8 * g + 4 * (lane >> 5);
+        if (d >= a.D) continue;
+        float4v x, y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = live ? dk[f][4 * g + j] : 0.f;
+          y[j] = live ? dv[f][4 * g + j] : 0.f;
+        }
+        *reinterpret_cast<float4v*>(p + d) = x;
+        *reinterpret_cast<float4v*>(p + n + d) = y;
+      }
   }
+}
+
+// part [splits][2][n] -> dk and dv [n], n a multiple of 8
+template <class E>
+__global__ __launch_bounds__(NTH) void packed_bwd_sum_kernel(
+    const float* __restrict__ part, short* __restrict__ dk,
+    short* __restrict__ dv, long n, int splits) {
+  const long i = ((long)blockIdx.x * NTH + threadIdx.x) * 8;
+  if (i >= 2 * n) return;
+  float v[8] = {};
+  for (int k = 0; k < splits; ++k) {
+    const float4v* p = reinterpret_cast<const float4v*>(part + 2 * k * n + i);
+    const float4v x = p[0], y = p[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] += x[j];
+      v[4 + j] += y[j];
+    }
+  }
+  short* out = i < n ? dk + i : dv + (i - n);
+  *reinterpret_cast<short8*>(out) = E::pack(v);
 }
 
 // ---- host --------------------------------------------------------------
@@ -599,16 +711,17 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   a.D = (int)q.size(2);
   a.window = (int)std::min<int64_t>(window, a.T);
   a.scale = (float)scale;
-  const long units = ((long)a.T / OWN + a.B + 1) * a.HK;
-  TORCH_CHECK(units * (a.H / a.HK) < (1L << 30),
+  const long slots = (long)a.T / OWN + a.B + 1;
+  TORCH_CHECK(slots * a.H < (1L << 30),
               "attn_packed: too many rows and heads");
-  a.units = (int)units;
+  a.slots = (int)slots;
+  a.splits = 1;
   return a;
 }
 
-#define PACKED_LAUNCH(KERNEL, REP)                                          \
+#define PACKED_LAUNCH(KERNEL, HEADS, REP)                                   \
   do {                                                                      \
-    const dim3 grid((a.units + 7) / 8 * 8 * (REP)), block(NTH);             \
+    const dim3 grid((a.slots * (HEADS) + 7) / 8 * 8 * (REP)), block(NTH);   \
     const auto st = stream.stream();                                        \
     if (bf && wide && causal)                                               \
       hipLaunchKernelGGL((KERNEL<BF, 128, true>), grid, block, 0, st, a);   \
@@ -646,7 +759,7 @@ std::vector<torch::Tensor> attn_packed_fwd(
   a.lse = lse.data_ptr<float>();
   auto stream = c10::cuda::getCurrentCUDAStream();
   const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
-  PACKED_LAUNCH(packed_fwd_kernel, a.H / a.HK);
+  PACKED_LAUNCH(packed_fwd_kernel, a.HK, a.H / a.HK);
   HIP_CHECK_LAST();
   return {o, lse};
 }
@@ -681,8 +794,29 @@ std::vector<torch::Tensor> attn_packed_bwd(
   a.drow = drow.data_ptr<float>();
   auto stream = c10::cuda::getCurrentCUDAStream();
   const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
-  PACKED_LAUNCH(packed_bwd_q_kernel, a.H / a.HK);
-  PACKED_LAUNCH(packed_bwd_kv_kernel, 1);
+  PACKED_LAUNCH(packed_bwd_q_kernel, a.HK, a.H / a.HK);
+  // two blocks of four waves on each of 256 CUs run at once: twice as many
+  // blocks even out their lengths
+  const int rep = a.H / a.HK;
+  while (a.splits < rep && (long)a.slots * a.HK * a.splits < 1024) {
+    do ++a.splits; while (rep % a.splits);
+  }
+  torch::Tensor part;
+  if (a.splits > 1) {
+    part = torch::empty({a.splits, 2, a.T, a.HK, a.D}, lse.options());
+    a.part = part.data_ptr<float>();
+  }
+  PACKED_LAUNCH(packed_bwd_kv_kernel, a.HK * a.splits, 1);
+  if (a.splits > 1) {
+    const long n = (long)a.T * a.HK * a.D;
+    const dim3 grid((unsigned)((2 * n / 8 + NTH - 1) / NTH));
+    if (bf)
+      hipLaunchKernelGGL((packed_bwd_sum_kernel<BF>), grid, dim3(NTH), 0,
+                         stream.stream(), a.part, a.dk, a.dv, n, a.splits);
+    else
+      hipLaunchKernelGGL((packed_bwd_sum_kernel<FH>), grid, dim3(NTH), 0,
+                         stream.stream(), a.part, a.dk, a.dv, n, a.splits);
+  }
   HIP_CHECK_LAST();
   return {dq, dk, dv};
 }
