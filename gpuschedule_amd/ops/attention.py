@@ -112,38 +112,6 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _ref_attention(q, k, v, causal)
 
 
-class _FlashAttnPackedFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, lengths, causal, window, scale):
-        ext = get_ext(required=True)
-        o, lse = ext.attn_packed_fwd(q, k, v, cu_seqlens, lengths, causal,
-                                     window, scale)
-        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens, lengths)
-        ctx.causal, ctx.window, ctx.scale = causal, window, scale
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        # probabilities are computed again from lse, nothing T x T is kept
-        ext = get_ext(required=True)
-        q, k, v, o, lse, cu_seqlens, lengths = ctx.saved_tensors
-        dq, dk, dv = ext.attn_packed_bwd(
-            q, k, v, o, _aligned_rows(do), lse, cu_seqlens, lengths,
-            ctx.causal, ctx.window, ctx.scale)
-        return dq, dk, dv, None, None, None, None, None
-
-
-def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
-    """x, or a copy of it where the kernels' 16-byte reads cannot follow
-    its strides.  (stride 0 is fine: every row is the same one.)"""
-    if x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 \
-            and x.data_ptr() % 16 == 0:
-        return x
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
-
-
 def _ref_attention_packed(q, k, v, cu_seqlens, lengths, causal, window,
                           scale):
     # fp32 composite; used on CPU
@@ -234,10 +202,7 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor,
             raise ValueError(f"flash_attention_packed: q, k and v must all "
                              f"be bf16 or fp16, got {q.dtype}, {k.dtype}, "
                              f"{v.dtype}")
-        return _FlashAttnPackedFn.apply(
-            _aligned_rows(q), _aligned_rows(k), _aligned_rows(v),
-            cu_seqlens.contiguous(),
-            None if lengths is None else lengths.contiguous(), causal,
-            window or 0, scale)
+        return get_ext(required=True).attn_packed(
+            q, k, v, cu_seqlens, lengths, causal, window or 0, scale)
     return _ref_attention_packed(q, k, v, cu_seqlens, lengths, causal,
                                  window, scale)

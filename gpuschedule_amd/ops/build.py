@@ -19,7 +19,8 @@ SOURCES = [os.path.join(HERE, "hip", f)
                      "optim.hip", "attention.hip", "bn.hip", "ce.hip",
                      "elementwise.hip", "embedding.hip",
                      "attention_packed.hip", "rope_axes.hip",
-                     "block_norm.hip", "clip.hip")]
+                     "block_norm.hip", "clip.hip",
+                     "packed_autograd.cpp")]
 EXT_NAME = "_hip_ops"
 
 

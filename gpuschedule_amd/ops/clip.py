@@ -7,7 +7,6 @@ scalar, and a captured step replays it.  CPU path: plain torch (tests).
 """
 from __future__ import annotations
 
-import math
 from typing import Iterable, List, Union
 
 import torch
@@ -15,21 +14,23 @@ import torch
 from ._ext import get_ext
 
 
-def _grads_of(parameters) -> List[torch.Tensor]:
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    seen, grads = set(), []
-    for p in parameters:
-        if p.grad is None or id(p) in seen:  # a tied weight counts once
-            continue
-        seen.add(id(p))
-        grads.append(p.grad.detach())
-    return grads
+def _with_grad(parameters):
+    """The parameters as a list, and the first gradient among them."""
+    params = ([parameters] if isinstance(parameters, torch.Tensor)
+              else list(parameters))
+    for p in params:
+        if p.grad is not None:
+            return params, p.grad
+    return params, None
+
+
+def _cpu_grads(params) -> List[torch.Tensor]:
+    # a tied weight counts once
+    return [p.grad for p in dict.fromkeys(params) if p.grad is not None]
 
 
 def _cpu_norm(grads) -> torch.Tensor:
-    total = sum(g.double().square().sum() for g in grads)
-    return torch.as_tensor(total).sqrt()
+    return sum(g.detach().double().square().sum() for g in grads).sqrt()
 
 
 def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]
@@ -39,13 +40,14 @@ def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]
 
     Gradients may mix bf16, fp16 and fp32.  They must be on one device,
     dense in memory (any order of dimensions), and must not share
-    memory.  Squares are summed in 64 bits."""
-    grads = _grads_of(parameters)
-    if not grads:
+    memory; a parameter that is named twice counts once.  Squares are
+    summed in 64 bits."""
+    params, any_grad = _with_grad(parameters)
+    if any_grad is None:
         return torch.zeros(())
-    if grads[0].is_cuda:
-        return get_ext(required=True).grad_norm_clip(grads, -1.0)
-    return _cpu_norm(grads).float()
+    if any_grad.is_cuda:
+        return get_ext(required=True).grad_norm_clip(params, -1.0)
+    return _cpu_norm(_cpu_grads(params)).float()
 
 
 @torch.no_grad()
@@ -59,16 +61,15 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]],
     gradients become 0 or NaN.  Check the returned norm to skip such a
     step."""
     max_norm = float(max_norm)
-    if math.isnan(max_norm) or max_norm < 0:
+    if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm must be >= 0, "
                          f"got {max_norm}")
-    grads = _grads_of(parameters)
-    if not grads:
+    params, any_grad = _with_grad(parameters)
+    if any_grad is None:
         return torch.zeros(())
-    if grads[0].is_cuda:
-        norm = get_ext(required=True).grad_norm_clip(grads, max_norm)
-        torch.autograd.graph.increment_version(grads)
-        return norm
+    if any_grad.is_cuda:
+        return get_ext(required=True).grad_norm_clip(params, max_norm)
+    grads = _cpu_grads(params)
     norm = _cpu_norm(grads)
     ratio = max_norm / (norm + 1e-6)
     if not ratio >= 1.0:

@@ -35,29 +35,6 @@ def fused_rope(x: torch.Tensor, cosb: torch.Tensor,
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
-class _RopeAxesFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, cosb, sinb, sections):
-        ext = get_ext(required=True)
-        ctx.save_for_backward(positions, cosb, sinb)
-        ctx.sections = sections
-        return tuple(ext.rope_axes(q, k, positions, cosb, sinb, sections,
-                                   False))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk):
-        ext = get_ext(required=True)
-        positions, cosb, sinb = ctx.saved_tensors
-        dq, dk = ext.rope_axes(_dense_rows(dq), _dense_rows(dk), positions,
-                               cosb, sinb, ctx.sections, True)
-        return dq, dk, None, None, None, None
-
-
-def _dense_rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 else x.contiguous()
-
-
 def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
                     positions: torch.Tensor, cosb: torch.Tensor,
                     sinb: torch.Tensor, sections: Sequence[int]):
@@ -103,9 +80,8 @@ def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
             raise ValueError("fused_rope_axes: all tensors must be on one "
                              "device")
     if q.is_cuda:
-        return _RopeAxesFn.apply(_dense_rows(q), _dense_rows(k),
-                                 positions.contiguous(), cosb.contiguous(),
-                                 sinb.contiguous(), sections)
+        return tuple(get_ext(required=True).rope_axes(
+            q, k, positions, cosb, sinb, sections))
     axis = torch.repeat_interleave(torch.arange(len(sections)),
                                    torch.tensor(sections))
     at = positions[axis].t().long()                        # [T, R/2]

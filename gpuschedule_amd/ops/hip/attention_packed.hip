@@ -661,7 +661,7 @@ __global__ __launch_bounds__(NTH) void packed_bwd_sum_kernel(
 
 bool rows_aligned(const torch::Tensor& t) {
   return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-         (size_t)t.data_ptr() % 16 == 0;
+         t.stride(0) < (1 << 24) && (size_t)t.data_ptr() % 16 == 0;
 }
 
 Args args_of(const torch::Tensor& q, const torch::Tensor& k,

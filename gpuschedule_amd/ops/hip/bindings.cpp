@@ -68,30 +68,20 @@ std::vector<torch::Tensor> bn_bwd(torch::Tensor dy, torch::Tensor x,
                                   torch::Tensor gamma, bool relu,
                                   bool want_dres,
                                   c10::optional<torch::Tensor> beta);
-std::vector<torch::Tensor> attn_packed_fwd(
-    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu,
-    c10::optional<torch::Tensor> lengths, bool causal, int64_t window,
-    double scale);
-std::vector<torch::Tensor> attn_packed_bwd(
-    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o,
-    torch::Tensor dout, torch::Tensor lse, torch::Tensor cu,
-    c10::optional<torch::Tensor> lengths, bool causal, int64_t window,
-    double scale);
-std::vector<torch::Tensor> rope_axes(torch::Tensor q, torch::Tensor k,
-                                     torch::Tensor pos, torch::Tensor cosb,
-                                     torch::Tensor sinb,
-                                     std::vector<int64_t> sections,
-                                     bool backward);
-std::vector<torch::Tensor> block_norm_fwd(torch::Tensor h, torch::Tensor x,
-                                          torch::Tensor w1, torch::Tensor w2,
-                                          c10::optional<torch::Tensor> gate,
-                                          double alpha, double eps,
-                                          bool train);
-std::vector<torch::Tensor> block_norm_bwd(
-    torch::Tensor dn, torch::Tensor ds, torch::Tensor h, torch::Tensor x,
-    torch::Tensor w1, torch::Tensor w2, c10::optional<torch::Tensor> gate,
-    torch::Tensor r1, torch::Tensor r2, double alpha);
-torch::Tensor grad_norm_clip(std::vector<torch::Tensor> grads,
+torch::Tensor attn_packed(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                          torch::Tensor cu,
+                          c10::optional<torch::Tensor> lengths, bool causal,
+                          int64_t window, double scale);
+std::vector<torch::Tensor> rope_axes_grad(torch::Tensor q, torch::Tensor k,
+                                          torch::Tensor pos,
+                                          torch::Tensor cosb,
+                                          torch::Tensor sinb,
+                                          std::vector<int64_t> sections);
+std::vector<torch::Tensor> block_norm(torch::Tensor h, torch::Tensor x,
+                                      torch::Tensor w1, torch::Tensor w2,
+                                      c10::optional<torch::Tensor> gate,
+                                      double alpha, double eps);
+torch::Tensor grad_norm_clip(std::vector<torch::Tensor> params,
                              double max_norm);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -142,16 +132,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("rstd"), py::arg("gamma"), py::arg("relu"),
         py::arg("want_dres"),
         py::arg("beta") = c10::optional<torch::Tensor>());
-  m.def("attn_packed_fwd", &attn_packed_fwd,
-        "attention over packed sequences, forward; returns (o, lse)");
-  m.def("attn_packed_bwd", &attn_packed_bwd,
-        "attention over packed sequences, backward: (dq, dk, dv)");
-  m.def("rope_axes", &rope_axes,
-        "rotate-half RoPE by token positions on several axes");
-  m.def("block_norm_fwd", &block_norm_fwd,
-        "post-norm + gate + residual + pre-norm forward: (n, s, r1, r2)");
-  m.def("block_norm_bwd", &block_norm_bwd,
-        "post-norm + gate + residual + pre-norm backward");
+  m.def("attn_packed", &attn_packed,
+        "attention over packed sequences, with its gradient");
+  m.def("rope_axes", &rope_axes_grad,
+        "rotate-half RoPE by token positions on several axes, with its "
+        "gradient");
+  m.def("block_norm", &block_norm,
+        "post-norm + gate + residual + pre-norm: (n, s), with its gradient");
   m.def("grad_norm_clip", &grad_norm_clip,
-        "global gradient norm; max_norm >= 0 also clips in place");
+        "global norm of parameters' gradients; max_norm >= 0 also clips them "
+        "in place");
 }

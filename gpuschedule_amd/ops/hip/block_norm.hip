@@ -299,10 +299,10 @@ Shape check(const torch::Tensor& h, const torch::Tensor& x,
   if (gate.has_value()) {
     const auto& g = *gate;
     TORCH_CHECK(g.is_contiguous() && g.dim() == 2 && g.size(1) == s.D &&
-                g.size(0) >= 1 && s.rows % g.size(0) == 0,
+                (s.rows == 0 || (g.size(0) >= 1 && s.rows % g.size(0) == 0)),
                 "block_norm: the gate must be contiguous [G, D], G a divisor "
                 "of the rows");
-    s.group = std::max<long>(s.rows / g.size(0), 1);
+    if (s.rows) s.group = s.rows / g.size(0);
     others.push_back(g);
   }
   for (const auto& o : others)

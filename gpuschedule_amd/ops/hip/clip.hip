@@ -181,12 +181,22 @@ __global__ __launch_bounds__(NT) void grad_clip_kernel(
   }
 }
 
-std::vector<GradTable> tables_of(const std::vector<torch::Tensor>& grads) {
-  constexpr long PIECE = 1L << 30;  // a longer tensor takes several entries
-  std::vector<std::pair<char*, char*>> spans;
-  std::vector<GradTable> tables;
-  for (const auto& g : grads) {
-    TORCH_CHECK(g.is_cuda() && g.device() == grads[0].device(),
+struct Grad {
+  char *begin, *end;
+  at::TensorImpl *param, *grad;
+  int type;
+};
+
+// The gradients of `params`, each once, in the order of their addresses.
+std::vector<Grad> grads_of(const std::vector<torch::Tensor>& params) {
+  std::vector<Grad> grads;
+  grads.reserve(params.size());
+  c10::optional<c10::Device> device;
+  for (const auto& p : params) {
+    const auto& g = p.grad();
+    if (!g.defined()) continue;
+    if (!device) device = g.device();
+    TORCH_CHECK(g.is_cuda() && g.device() == *device,
                 "grad_norm: all gradients must be on one GPU");
     TORCH_CHECK(g.layout() == torch::kStrided && g.is_non_overlapping_and_dense(),
                 "grad_norm: gradients must be dense in memory");
@@ -194,10 +204,34 @@ std::vector<GradTable> tables_of(const std::vector<torch::Tensor>& grads) {
     TORCH_CHECK(st == torch::kBFloat16 || st == torch::kHalf ||
                     st == torch::kFloat32,
                 "grad_norm: gradients must be bf16, fp16 or fp32, got ", st);
-    const long n = g.numel(), size = g.element_size();
-    if (n == 0) continue;
-    char* p = (char*)g.data_ptr();
-    spans.emplace_back(p, p + n * size);
+    if (g.numel() == 0) continue;
+    char* at = (char*)g.data_ptr();
+    grads.push_back({at, at + g.nbytes(), p.unsafeGetTensorImpl(),
+                     g.unsafeGetTensorImpl(),
+                     st == torch::kBFloat16 ? BF16
+                                            : st == torch::kHalf ? F16 : F32});
+  }
+  std::sort(grads.begin(), grads.end(), [](const Grad& a, const Grad& b) {
+    return a.begin < b.begin;
+  });
+  // a tied weight counts once
+  grads.erase(std::unique(grads.begin(), grads.end(),
+                          [](const Grad& a, const Grad& b) {
+                            return a.param == b.param;
+                          }),
+              grads.end());
+  // two blocks would scale shared memory at once
+  for (size_t i = 1; i < grads.size(); ++i)
+    TORCH_CHECK(grads[i].begin >= grads[i - 1].end,
+                "grad_norm: two gradients share memory");
+  return grads;
+}
+
+std::vector<GradTable> tables_of(const std::vector<Grad>& grads) {
+  constexpr long PIECE = 1L << 30;  // a longer tensor takes several entries
+  std::vector<GradTable> tables;
+  for (const auto& g : grads) {
+    const long size = g.type == F32 ? 4 : 2, n = (g.end - g.begin) / size;
     for (long off = 0; off < n; off += PIECE) {
       if (tables.empty() || tables.back().count == MAX_T) {
         tables.emplace_back();
@@ -207,39 +241,39 @@ std::vector<GradTable> tables_of(const std::vector<torch::Tensor>& grads) {
       auto& t = tables.back();
       const long m = std::min(PIECE, n - off);
       const int i = t.count++;
-      t.ptr[i] = p + off * size;
+      t.ptr[i] = g.begin + off * size;
       t.numel[i] = (unsigned)m;
-      t.type[i] = st == torch::kBFloat16 ? BF16 : st == torch::kHalf ? F16 : F32;
+      t.type[i] = g.type;
       t.first[i + 1] = t.first[i] + (unsigned)((m + CHUNK - 1) / CHUNK);
     }
   }
-  // two blocks would scale shared memory at once
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK(spans[i].first >= spans[i - 1].second,
-                "grad_norm: two gradients share memory");
   return tables;
 }
 
 }  // namespace
 
-// The norm of all tensors, as fp32 [].  max_norm >= 0: they are scaled in
-// place so that their norm is at most that.  max_norm < 0: norm only.
-torch::Tensor grad_norm_clip(std::vector<torch::Tensor> grads,
+// The norm of the gradients of `params`, as fp32 [] (those without one are
+// left out).  max_norm >= 0: they are scaled in place so that their norm is
+// at most that.  max_norm < 0: norm only.
+torch::Tensor grad_norm_clip(std::vector<torch::Tensor> params,
                              double max_norm) {
-  TORCH_CHECK(!grads.empty(), "grad_norm: no gradients");
+  c10::optional<torch::Tensor> any;
+  for (const auto& p : params)
+    if (p.grad().defined()) any = p.grad();
+  TORCH_CHECK(any, "grad_norm: no gradients");
+  const auto grads = grads_of(params);
   const auto tables = tables_of(grads);
-  const c10::cuda::CUDAGuard guard(grads[0].device());
+  const c10::cuda::CUDAGuard guard(any->device());
   auto stream = c10::cuda::getCurrentCUDAStream();
-  auto norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+  const auto opt = torch::TensorOptions().device(any->device());
+  auto norm = torch::empty({}, opt.dtype(torch::kFloat32));
   std::vector<int> grid;
   int parts = 0;
   for (const auto& t : tables) {
     grid.push_back((int)std::min<unsigned>(t.first[t.count], MAX_BLOCKS));
     parts += grid.back();
   }
-  auto part = torch::empty({std::max(parts, 1)},
-                           grads[0].options().dtype(torch::kFloat64));
+  auto part = torch::empty({std::max(parts, 1)}, opt.dtype(torch::kFloat64));
   double* pp = part.data_ptr<double>();
   int at = 0;
   for (size_t i = 0; i < tables.size(); ++i) {
@@ -255,6 +289,9 @@ torch::Tensor grad_norm_clip(std::vector<torch::Tensor> grads,
       hipLaunchKernelGGL(grad_clip_kernel, dim3(grid[i]), dim3(NT), 0,
                          stream.stream(), tables[i], pp, parts, max_norm,
                          i == 0 ? norm.data_ptr<float>() : nullptr);
+  if (max_norm >= 0)
+    for (const auto& g : grads)
+      if (!g.grad->is_inference()) g.grad->bump_version();
   HIP_CHECK_LAST();
   return norm;
 }

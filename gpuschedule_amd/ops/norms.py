@@ -106,30 +106,6 @@ class FusedRMSNorm(nn.Module):
         return f"{self.dim}, eps={self.eps}"
 
 
-class _BlockNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, h, x, post_weight, pre_weight, gate, alpha, eps):
-        ext = get_ext(required=True)
-        train = any(ctx.needs_input_grad)
-        n, s, r1, r2 = ext.block_norm_fwd(h, x, post_weight, pre_weight,
-                                          gate, alpha, eps, train)
-        # the sum is computed again in backward, from h and x
-        ctx.save_for_backward(h, x, post_weight, pre_weight, gate, r1, r2)
-        ctx.alpha = alpha
-        return n, s
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dn, ds):
-        ext = get_ext(required=True)
-        h, x, w1, w2, gate, r1, r2 = ctx.saved_tensors
-        dh, dx, dw1, dw2, dg = ext.block_norm_bwd(
-            dn.contiguous(), ds.contiguous(), h, x, w1, w2, gate, r1, r2,
-            ctx.alpha)
-        return (dh, dx, dw1, dw2, dg if gate is not None else None, None,
-                None)
-
-
 def fused_block_norm(h: torch.Tensor, x: torch.Tensor,
                      post_weight: torch.Tensor, pre_weight: torch.Tensor,
                      gate: Optional[torch.Tensor] = None,
@@ -182,14 +158,8 @@ def fused_block_norm(h: torch.Tensor, x: torch.Tensor,
         s = residual_scale * xf + g * (z * post_weight.float())
         n = s * torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + eps)
         return (n * pre_weight.float()).to(h.dtype), s.to(h.dtype)
-    if gate is not None:
-        gate = gate.reshape(-1, D).contiguous()
-        if h.numel() == 0:
-            gate = None
-    return _BlockNormFn.apply(h.contiguous(), x.contiguous(),
-                              post_weight.contiguous(),
-                              pre_weight.contiguous(), gate,
-                              float(residual_scale), float(eps))
+    return tuple(get_ext(required=True).block_norm(
+        h, x, post_weight, pre_weight, gate, residual_scale, eps))
 
 
 class FusedBlockNorm(nn.Module):
