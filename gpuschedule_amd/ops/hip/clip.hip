@@ -37,7 +37,9 @@ template <int TYPE> struct Elem;
 template <> struct Elem<BF16> {
   using T = short;
   static __device__ float up(T v) { return bf16_to_f32(v); }
-  static __device__ T down(float f) { return f32_to_bf16(f); }
+  static __device__ T down(float f) {
+    return __builtin_bit_cast(short, (__bf16)f);
+  }
 };
 template <> struct Elem<F16> {
   using T = _Float16;

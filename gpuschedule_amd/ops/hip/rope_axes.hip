@@ -41,7 +41,7 @@ template <> __device__ __forceinline__ float up(short v) {
 }
 template <class T> __device__ __forceinline__ T down(float f) { return (T)f; }
 template <> __device__ __forceinline__ short down(float f) {
-  return f32_to_bf16(f);
+  return __builtin_bit_cast(short, (__bf16)f);
 }
 
 // 8 values at any alignment of their own type
