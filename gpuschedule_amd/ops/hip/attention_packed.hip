@@ -92,6 +92,7 @@ struct Args {
 };
 
 __device__ const uint4v kZeros = {0, 0, 0, 0};
+__device__ const float kInf = INFINITY;
 
 // ---- which rows --------------------------------------------------------
 
@@ -149,6 +150,10 @@ template <int DP> __device__ __forceinline__ int mix(int r) {
   return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
 }
 
+// Every buffer is an array of its own and every tile names the ones that it
+// reads and fills: only then does the compiler see that a read need not wait
+// for the tile that is still on its way.
+
 // Rows of p (stride `ld`) go to LDS without passing registers, 16 bytes a
 // lane.  One offset a lane serves all of its pieces: they are NTH / NCH rows
 // apart, at which the swizzle repeats, so the rest of the address is uniform.
@@ -190,34 +195,50 @@ __device__ __forceinline__ void stage(const short* p, long ld, unsigned off,
   }
 }
 
-// A operand from rows: row r0 + l % 32, values 16 kk + 8 (l / 32) + 0..7.
-template <int DP>
-__device__ __forceinline__ short8 rows_of(const char* tile, int r0, int kk,
-                                          int lane) {
-  const int r = r0 + (lane & 31), c = 2 * kk + (lane >> 5);
-  return *reinterpret_cast<const short8*>(tile + r * DP * 2 +
-                                          ((c ^ mix<DP>(r)) << 4));
-}
+// Where a lane reads in a tile.  The swizzle repeats after 16 rows, and the
+// steps along a row change other bits of the chunk than the lane does: both
+// kinds of reads are one offset of the lane, one XOR with a constant and a
+// constant more.
+template <int DP> struct Lane {
+  unsigned row, col[2];
 
-// A operand from columns: value 32 f + l % 32 of 8 rows, in the order of an
-// accumulator: rows r0 + 4 (l / 32) + 0..3 and r0 + 8 + 4 (l / 32) + 0..3.
-// In a transposing read the 16 lanes of a group name 4 rows of 16 values,
-// 4 values each, and lane j of the group gets value j of the 4 rows.
-template <int DP>
-__device__ __forceinline__ short8 cols_of(const char* tile, int r0, int f,
-                                          int lane) {
-  short4v part[2];
+  __device__ __forceinline__ explicit Lane(int lane) {
+    const int r = lane & 31;
+    row = r * DP * 2 + (((lane >> 5) ^ mix<DP>(r)) << 4);
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int j = lane & 15;
-    const int r = r0 + 8 * b + 4 * (lane >> 5) + (j >> 2);
-    const int c = 4 * f + (lane >> 4 & 1) * 2 + (j >> 1 & 1);
-    const char* at = tile + r * DP * 2 + ((c ^ mix<DP>(r)) << 4) + (j & 1) * 8;
-    part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) short4v*)at);
+    for (int b = 0; b < 2; ++b) {
+      const int j = lane & 15, rb = 8 * b + 4 * (lane >> 5) + (j >> 2);
+      const int c = (lane >> 4 & 1) * 2 + (j >> 1 & 1);
+      col[b] = rb * DP * 2 + ((c ^ mix<DP>(rb)) << 4) + (j & 1) * 8;
+    }
   }
-  return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-}
+  // Forget what was worked out from the offsets: registers are dearer than
+  // the XORs.
+  __device__ __forceinline__ void again() {
+    asm volatile("" : "+v"(row), "+v"(col[0]), "+v"(col[1]));
+  }
+  // A (or B) operand from rows: row r0 + l % 32, values 16 kk + 8 (l / 32)
+  // + 0..7.
+  __device__ __forceinline__ short8 rows(const char* tile, int r0,
+                                         int kk) const {
+    return *reinterpret_cast<const short8*>(tile + (row ^ kk << 5) +
+                                            r0 * DP * 2);
+  }
+  // A operand from columns: value 32 f + l % 32 of 8 rows, in the order of
+  // an accumulator: r0 + 4 (l / 32) + 0..3 and r0 + 8 + 4 (l / 32) + 0..3.
+  // In a transposing read the 16 lanes of a group name 4 rows of 16 values,
+  // 4 values each, and lane j of the group gets value j of the 4 rows.
+  __device__ __forceinline__ short8 cols(const char* tile, int r0,
+                                         int f) const {
+    short4v part[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) short4v*)(
+              tile + (col[b] ^ f << 6) + r0 * DP * 2));
+    return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
 
 // B operand straight from global memory: row of this lane, DP / 16 steps.
 template <int DP>
@@ -290,10 +311,14 @@ __device__ __forceinline__ bool seen(const Args& a, int key, int row,
 
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
-  __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char k1[TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char v1[TILE * DP * 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.H / a.HK;
+  Lane<DP> at_lane(lane);
   int kvh, slot, sub, row0;
   Seq s;
   if (!unit_of(a, a.HK, rep, CAUSAL, kvh, slot, sub)) return;
@@ -317,21 +342,17 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
     const unsigned koff = stage_offset<DP>(a.k_t);
     const unsigned voff = stage_offset<DP>(a.v_t);
     const int end = CAUSAL ? min(s.len, row0 + OWN) : s.len;
-    const int t0 = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
     const int t1 = (end + TILE - 1) / TILE;
     const float sl2 = a.scale * kLog2e;
-    stage<DP, TILE>(kp, a.k_t, koff, t0 * TILE, s.len, a.D, lds[0]);
-    stage<DP, TILE>(vp, a.v_t, voff, t0 * TILE, s.len, a.D, lds[1]);
-    __syncthreads();
-    int buf = 0;
-    for (int t = t0; t < t1; ++t, buf ^= 2) {
+    auto fetch = [&](int t, char* k, char* v) {
+      stage<DP, TILE>(kp, a.k_t, koff, t * TILE, s.len, a.D, k);
+      stage<DP, TILE>(vp, a.v_t, voff, t * TILE, s.len, a.D, v);
+    };
+    // One tile, while the next one is on its way to the other buffers.
+    auto tile = [&](int t, const char* kt, const char* vt, char* kn, char* vn)
+        __attribute__((always_inline)) {
       const int kv0 = t * TILE;
-      const char *kt = lds[buf], *vt = lds[buf + 1];
-      if (t + 1 < t1) {
-        stage<DP, TILE>(kp, a.k_t, koff, kv0 + TILE, s.len, a.D, lds[buf ^ 2]);
-        stage<DP, TILE>(vp, a.v_t, voff, kv0 + TILE, s.len, a.D,
-                        lds[(buf ^ 2) + 1]);
-      }
+      if (t + 1 < t1) fetch(t + 1, kn, vn);
       const int what = sees<CAUSAL>(a, kv0, first, s.len);
       if (what) {
         float16v sc[2];
@@ -340,7 +361,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           sc[kb] = (float16v)(0.f);
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk)
-            sc[kb] = E::mfma(rows_of<DP>(kt, 32 * kb, kk, lane), q[kk], sc[kb]);
+            sc[kb] = E::mfma(at_lane.rows(kt, 32 * kb, kk), q[kk], sc[kb]);
         }
         if (what == 1) {
 #pragma unroll
@@ -372,6 +393,11 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
             for (int i = 0; i < 16; ++i) o[f][i] *= alpha;
         }
         const float ref = m == kNone ? 0.f : m;
+        // A wave that has its probabilities goes before one that has not:
+        // that keeps the two waves of a SIMD in different phases, one in
+        // matrix and one in vector instructions (297 us without, 277 with,
+        // 8192 tokens of 16/4 heads of 128).
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           float p[8];
@@ -385,10 +411,18 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           const short8 pb = E::pack(p);
 #pragma unroll
           for (int f = 0; f < DP / 32; ++f)
-            o[f] = E::mfma(cols_of<DP>(vt, 16 * ks, f, lane), pb, o[f]);
+            o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pb, o[f]);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
       __syncthreads();
+    };
+    int t = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
+    fetch(t, k0, v0);
+    __syncthreads();
+    for (; t < t1; ++t) {
+      tile(t, k0, v0, k1, v1);
+      if (++t < t1) tile(t, k1, v1, k0, v0);
     }
   }
   l += other_half(l);
@@ -405,10 +439,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
-  __shared__ __attribute__((aligned(16))) char lds[4][TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char k1[TILE * DP * 2];
+  __shared__ __attribute__((aligned(16))) char v1[TILE * DP * 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.H / a.HK;
+  Lane<DP> at_lane(lane);
   int kvh, slot, sub, row0;
   Seq s;
   if (!unit_of(a, a.HK, rep, CAUSAL, kvh, slot, sub)) return;
@@ -444,21 +482,16 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     const unsigned koff = stage_offset<DP>(a.k_t);
     const unsigned voff = stage_offset<DP>(a.v_t);
     const int end = CAUSAL ? min(s.len, row0 + OWN) : s.len;
-    const int t0 = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
     const int t1 = (end + TILE - 1) / TILE;
     const float sl2 = a.scale * kLog2e;
-    stage<DP, TILE>(kp, a.k_t, koff, t0 * TILE, s.len, a.D, lds[0]);
-    stage<DP, TILE>(vp, a.v_t, voff, t0 * TILE, s.len, a.D, lds[1]);
-    __syncthreads();
-    int buf = 0;
-    for (int t = t0; t < t1; ++t, buf ^= 2) {
+    auto fetch = [&](int t, char* k, char* v) {
+      stage<DP, TILE>(kp, a.k_t, koff, t * TILE, s.len, a.D, k);
+      stage<DP, TILE>(vp, a.v_t, voff, t * TILE, s.len, a.D, v);
+    };
+    auto tile = [&](int t, const char* kt, const char* vt, char* kn, char* vn)
+        __attribute__((always_inline)) {
       const int kv0 = t * TILE;
-      const char *kt = lds[buf], *vt = lds[buf + 1];
-      if (t + 1 < t1) {
-        stage<DP, TILE>(kp, a.k_t, koff, kv0 + TILE, s.len, a.D, lds[buf ^ 2]);
-        stage<DP, TILE>(vp, a.v_t, voff, kv0 + TILE, s.len, a.D,
-                        lds[(buf ^ 2) + 1]);
-      }
+      if (t + 1 < t1) fetch(t + 1, kn, vn);
       const int what = sees<CAUSAL>(a, kv0, first, s.len);
       if (what) {
 #pragma unroll
@@ -466,8 +499,8 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
           float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
-            sc = E::mfma(rows_of<DP>(kt, 32 * kb, kk, lane), q[kk], sc);
-            dp = E::mfma(rows_of<DP>(vt, 32 * kb, kk, lane), dO[kk], dp);
+            sc = E::mfma(at_lane.rows(kt, 32 * kb, kk), q[kk], sc);
+            dp = E::mfma(at_lane.rows(vt, 32 * kb, kk), dO[kk], dp);
           }
           if (what == 1) {
 #pragma unroll
@@ -487,12 +520,19 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
             const short8 b = E::pack(ds + 8 * ks);
 #pragma unroll
             for (int f = 0; f < DP / 32; ++f)
-              dq[f] = E::mfma(cols_of<DP>(kt, 32 * kb + 16 * ks, f, lane), b,
+              dq[f] = E::mfma(at_lane.cols(kt, 32 * kb + 16 * ks, f), b,
                               dq[f]);
           }
         }
       }
       __syncthreads();
+    };
+    int t = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
+    fetch(t, k0, v0);
+    __syncthreads();
+    for (; t < t1; ++t) {
+      tile(t, k0, v0, k1, v1);
+      if (++t < t1) tile(t, k1, v1, k0, v0);
     }
   }
   if (row < s.rows)
@@ -507,18 +547,24 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 //
 // Registers are what this kernel is short of: two accumulators of 32 x DP
 // and a fragment of k take 160 of the 256 that two waves on a SIMD leave, so
-// v stays in LDS, and query tiles are 32 rows.
+// v stays in LDS, query tiles are 32 rows, and LDS offsets are worked out
+// again for each tile (a spilled register in this loop doubles its time).
 
 constexpr int QT = 32;
 
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char own_v[OWN * DP * 2];
-  __shared__ __attribute__((aligned(16))) char lds[4][QT * DP * 2];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][QT];
+  __shared__ __attribute__((aligned(16))) char q0[QT * DP * 2];
+  __shared__ __attribute__((aligned(16))) char d0[QT * DP * 2];
+  __shared__ __attribute__((aligned(16))) char q1[QT * DP * 2];
+  __shared__ __attribute__((aligned(16))) char d1[QT * DP * 2];
+  __shared__ __attribute__((aligned(16))) float s0[2 * QT];
+  __shared__ __attribute__((aligned(16))) float s1[2 * QT];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.H / a.HK, mine = rep / a.splits;
+  Lane<DP> at_lane(lane);
   int vh, slot, none, row0;
   Seq s;
   if (!unit_of(a, a.HK * a.splits, 1, false, vh, slot, none)) return;
@@ -546,70 +592,80 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
     const int t1 = (end + QT - 1) / QT;
     const int last = first + 31;
     const float sl2 = a.scale * kLog2e;
-    auto fetch = [&](int head, int t, int buf) {
+    // a query tile, its lse and its D
+    auto fetch = [&](int head, int t, char* q, char* d, float* st) {
       stage<DP, QT>(a.q + s.begin * a.q_t + head * a.q_h, a.q_t, qoff, t * QT,
-                    s.len, a.D, lds[2 * buf]);
+                    s.len, a.D, q);
       stage<DP, QT>(a.dout + s.begin * a.d_t + head * a.d_h, a.d_t, doff,
-                    t * QT, s.len, a.D, lds[2 * buf + 1]);
-      if (threadIdx.x < QT) {
-        const int row = t * QT + threadIdx.x;
-        const long e = (long)head * a.T + s.begin + row;
-        const bool ok = row < s.len;
-        stat[buf][0][threadIdx.x] = ok ? a.lse[e] : INFINITY;
-        stat[buf][1][threadIdx.x] = ok ? a.drow[e] : 0.f;
+                    t * QT, s.len, a.D, d);
+      if (wave == 0) {
+        const int r = t * QT + (lane & 31);
+        const long e = (long)head * a.T + s.begin + r;
+        const float* src = lane < 32 ? a.lse + e : a.drow + e;
+        if (r >= s.len) src = lane < 32 ? &kInf : (const float*)&kZeros;
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) unsigned*)src,
+            (__attribute__((address_space(3))) unsigned*)st, 4, 0, 0);
       }
     };
-    fetch(h0, t0, 0);
-    __syncthreads();
-    int buf = 0;
-    for (int head = h0; head < h0 + mine; ++head)
-      for (int t = t0; t < t1; ++t, buf ^= 1) {
-        const int q0 = t * QT;
-        if (t + 1 < t1) fetch(head, t + 1, buf ^ 1);
-        else if (head + 1 < h0 + mine) fetch(head + 1, t0, buf ^ 1);
-        const char *qt = lds[2 * buf], *dt = lds[2 * buf + 1];
-        if ((!CAUSAL || q0 + QT > first) && first < s.len &&
-            (!a.window || q0 <= last + a.window - 1)) {
-          float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
+    int head = h0, t = t0;
+    auto tile = [&](const char* qt, const char* dt, const float* st, char* qn,
+                    char* dn, float* sn) __attribute__((always_inline)) {
+      const int r0 = t * QT;
+      at_lane.again();
+      if (++t == t1) {
+        t = t0;
+        ++head;
+      }
+      if (head < h0 + mine) fetch(head, t, qn, dn, sn);
+      if ((!CAUSAL || r0 + QT > first) && first < s.len &&
+          (!a.window || r0 <= last + a.window - 1)) {
+        float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
 #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            sc = E::mfma(rows_of<DP>(qt, 0, kk, lane), k[kk], sc);
-            dp = E::mfma(rows_of<DP>(dt, 0, kk, lane),
-                         rows_of<DP>(own_v, wave * 32, kk, lane), dp);
-          }
-          if ((CAUSAL && q0 < last) ||
-              (a.window && q0 + QT - 1 >= first + a.window)) {
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          sc = E::mfma(at_lane.rows(qt, 0, kk), k[kk], sc);
+          dp = E::mfma(at_lane.rows(dt, 0, kk),
+                       at_lane.rows(own_v, wave * 32, kk), dp);
+        }
+        if ((CAUSAL && r0 < last) ||
+            (a.window && r0 + QT - 1 >= first + a.window)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int row = q0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-              if (!seen<CAUSAL>(a, key, row, s.len)) sc[i] = kNone;
-            }
-          }
-          float p[16], ds[16];
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int r = 8 * g + 4 * (lane >> 5);
-            const float4v ls = *reinterpret_cast<float4v*>(&stat[buf][0][r]);
-            const float4v dr = *reinterpret_cast<float4v*>(&stat[buf][1][r]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int i = 4 * g + j;
-              p[i] = exp2_of(sc[i] * sl2 - ls[j]);
-              ds[i] = p[i] * (dp[i] * a.scale - dr[j]);
-            }
-          }
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            const short8 pb = E::pack(p + 8 * ks), sb = E::pack(ds + 8 * ks);
-#pragma unroll
-            for (int f = 0; f < DP / 32; ++f) {
-              dv[f] = E::mfma(cols_of<DP>(dt, 16 * ks, f, lane), pb, dv[f]);
-              dk[f] = E::mfma(cols_of<DP>(qt, 16 * ks, f, lane), sb, dk[f]);
-            }
+          for (int i = 0; i < 16; ++i) {
+            const int row = r0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+            if (!seen<CAUSAL>(a, key, row, s.len)) sc[i] = kNone;
           }
         }
-        __syncthreads();
+        float p[16], ds[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int r = 8 * g + 4 * (lane >> 5);
+          const float4v ls = *reinterpret_cast<const float4v*>(st + r);
+          const float4v dr = *reinterpret_cast<const float4v*>(st + QT + r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * g + j;
+            p[i] = exp2_of(sc[i] * sl2 - ls[j]);
+            ds[i] = p[i] * (dp[i] * a.scale - dr[j]);
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const short8 pb = E::pack(p + 8 * ks), sb = E::pack(ds + 8 * ks);
+#pragma unroll
+          for (int f = 0; f < DP / 32; ++f) {
+            dv[f] = E::mfma(at_lane.cols(dt, 16 * ks, f), pb, dv[f]);
+            dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sb, dk[f]);
+          }
+        }
       }
+      __syncthreads();
+    };
+    fetch(head, t, q0, d0, s0);
+    __syncthreads();
+    while (head < h0 + mine) {
+      tile(q0, d0, s0, q1, d1, s1);
+      if (head < h0 + mine) tile(q1, d1, s1, q0, d0, s0);
+    }
   }
   if (key >= s.rows) return;
   if (a.splits == 1) {
