@@ -159,7 +159,7 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor,
 
     ``causal``: a row sees its own and earlier rows; ``window`` (causal
     only): of those the last ``window``, its own among them.  ``scale``
-    defaults to 1/sqrt(D).
+    (positive) defaults to 1/sqrt(D).
 
     Returns o [T, H, D], contiguous.  Rows that are no tokens get zeros,
     in o and in the gradients, whatever they hold.  An infinity or NaN
@@ -194,8 +194,9 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor,
         raise ValueError("flash_attention_packed: window must be at least "
                          "1, and needs causal")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"flash_attention_packed: scale is {scale}")
+    if not 1e-30 < scale < 1e30:
+        raise ValueError(f"flash_attention_packed: scale must be positive, "
+                         f"got {scale}")
     if q.is_cuda:
         if q.dtype not in (torch.bfloat16, torch.float16) \
                 or k.dtype != q.dtype or v.dtype != q.dtype:

@@ -76,6 +76,7 @@ struct FH {
   }
 };
 
+
 constexpr int NW = 4, NTH = NW * 64;
 constexpr int TILE = 64;           // rows of a staged tile
 constexpr int OWN = 32 * NW;       // rows that a block owns: 32 a wave
@@ -83,7 +84,7 @@ constexpr int OWN = 32 * NW;       // rows that a block owns: 32 a wave
 struct Args {
   const short *q, *k, *v, *o, *dout;
   short *out, *dq, *dk, *dv;
-  float *lse, *drow;               // [H, T]; lse in units of log 2
+  float *lse, *drow;               // [H, T]: -log sum exp(s) / scale, and -D
   float* part;                     // [splits][dk, dv][T, HK, D]
   const int *cu, *lengths;         // lengths may be null
   long q_t, q_h, k_t, k_h, v_t, v_h, d_t, d_h;  // strides; d: dout
@@ -92,7 +93,7 @@ struct Args {
 };
 
 __device__ const uint4v kZeros = {0, 0, 0, 0};
-__device__ const float kInf = INFINITY;
+__device__ const float kNoLse = -INFINITY;
 
 // ---- which rows --------------------------------------------------------
 
@@ -269,6 +270,28 @@ __device__ __forceinline__ void put_rows(short* p, bool live, int D, int lane,
     }
 }
 
+// The order of instructions in the block of code that a call ends: so many
+// LDS reads, matrix or vector instructions next.
+template <int N> __device__ __forceinline__ void sched_reads() {
+  __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
+}
+template <int N> __device__ __forceinline__ void sched_mfma() {
+  __builtin_amdgcn_sched_group_barrier(0x8, N, 0);
+}
+template <int N> __device__ __forceinline__ void sched_vector() {
+  __builtin_amdgcn_sched_group_barrier(0x402, N, 0);
+}
+// N times: a product, READS reads, VECTOR vector instructions.
+template <int N, int READS, int VECTOR>
+__device__ __forceinline__ void order() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    sched_mfma<1>();
+    sched_reads<READS>();
+    if constexpr (VECTOR > 0) sched_vector<VECTOR>();
+  }
+}
+
 // The other half's value (lane l ^ 32).
 __device__ __forceinline__ float other_half(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(
@@ -413,6 +436,12 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           for (int f = 0; f < DP / 32; ++f)
             o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pb, o[f]);
         }
+        // the first probabilities, then a few more beside each product, whose
+        // fragments are read two products ahead
+        sched_reads<4>();
+        sched_vector<36>();
+        order<DP / 8 - 2, 2, 6>();
+        sched_mfma<2>();
         __builtin_amdgcn_s_setprio(0);
       }
       __syncthreads();
@@ -431,7 +460,8 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
                     o);
     // a row without keys: exp(s - inf) is 0 in backward
     if (lane < 32)
-      a.lse[(long)head * a.T + at] = live ? m + log2f(l) : INFINITY;
+      a.lse[(long)head * a.T + at] =
+          live ? -(m + log2f(l)) / (a.scale * kLog2e) : kNone;
   }
 }
 
@@ -473,10 +503,10 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           dr += E::up(ov[kk][j]) * E::up(dO[kk][j]);
-      dr = (dr + other_half(dr)) * a.scale;
+      dr += other_half(dr);
     }
-    const float lse = live ? a.lse[(long)head * a.T + at] : INFINITY;
-    if (live && lane < 32) a.drow[(long)head * a.T + at] = dr;
+    const float lse =
+        live ? -a.lse[(long)head * a.T + at] * (a.scale * kLog2e) : INFINITY;
     const short* kp = a.k + s.begin * a.k_t + kvh * a.k_h;
     const short* vp = a.v + s.begin * a.v_t + kvh * a.v_h;
     const unsigned koff = stage_offset<DP>(a.k_t);
@@ -488,10 +518,36 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
       stage<DP, TILE>(kp, a.k_t, koff, t * TILE, s.len, a.D, k);
       stage<DP, TILE>(vp, a.v_t, voff, t * TILE, s.len, a.D, v);
     };
+    int t = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
+    // D = dO.o carries the rounding of o, and of the probabilities that went
+    // into it: next to nothing where many keys share a row, but with few it
+    // is half of the error of dQ and dK.  Where a block's rows see no more
+    // keys than its two buffers hold, D is the sum of p dP instead.
+    const bool few = t1 - t <= 2;
+    auto dots = [&](int t, const char* kt, const char* vt)
+        __attribute__((always_inline)) {
+      const int kv0 = t * TILE;
+      if (!sees<CAUSAL>(a, kv0, first, s.len)) return;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          sc = E::mfma(at_lane.rows(kt, 32 * kb, kk), q[kk], sc);
+          dp = E::mfma(at_lane.rows(vt, 32 * kb, kk), dO[kk], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kv0 + 32 * kb + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+          if (seen<CAUSAL>(a, key, row, s.len))
+            dr += exp2_of(sc[i] * sl2 - lse) * dp[i];
+        }
+      }
+    };
     auto tile = [&](int t, const char* kt, const char* vt, char* kn, char* vn)
         __attribute__((always_inline)) {
       const int kv0 = t * TILE;
-      if (t + 1 < t1) fetch(t + 1, kn, vn);
+      if (!few && t + 1 < t1) fetch(t + 1, kn, vn);
       const int what = sees<CAUSAL>(a, kv0, first, s.len);
       if (what) {
 #pragma unroll
@@ -527,9 +583,17 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
       }
       __syncthreads();
     };
-    int t = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
     fetch(t, k0, v0);
+    if (few && t + 1 < t1) fetch(t + 1, k1, v1);
     __syncthreads();
+    if (few) {
+      dr = 0.f;
+      dots(t, k0, v0);
+      if (t + 1 < t1) dots(t + 1, k1, v1);
+      dr += other_half(dr);
+    }
+    if (live && lane < 32) a.drow[(long)head * a.T + at] = -dr;
+    dr *= a.scale;
     for (; t < t1; ++t) {
       tile(t, k0, v0, k1, v1);
       if (++t < t1) tile(t, k1, v1, k0, v0);
@@ -602,25 +666,36 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
         const int r = t * QT + (lane & 31);
         const long e = (long)head * a.T + s.begin + r;
         const float* src = lane < 32 ? a.lse + e : a.drow + e;
-        if (r >= s.len) src = lane < 32 ? &kInf : (const float*)&kZeros;
+        if (r >= s.len) src = lane < 32 ? &kNoLse : (const float*)&kZeros;
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) unsigned*)src,
             (__attribute__((address_space(3))) unsigned*)st, 4, 0, 0);
       }
     };
-    int head = h0, t = t0;
+    int head = h0, t = t1 - 1;
     auto tile = [&](const char* qt, const char* dt, const float* st, char* qn,
                     char* dn, float* sn) __attribute__((always_inline)) {
       const int r0 = t * QT;
       at_lane.again();
-      if (++t == t1) {
-        t = t0;
+      if (--t < t0) {
+        t = t1 - 1;
         ++head;
       }
       if (head < h0 + mine) fetch(head, t, qn, dn, sn);
       if ((!CAUSAL || r0 + QT > first) && first < s.len &&
           (!a.window || r0 <= last + a.window - 1)) {
-        float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
+        float16v sc, dp;           // begin as -lse and -D of their rows
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int r = 8 * g + 4 * (lane >> 5);
+          const float4v ls = *reinterpret_cast<const float4v*>(st + r);
+          const float4v dr = *reinterpret_cast<const float4v*>(st + QT + r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[4 * g + j] = ls[j];
+            dp[4 * g + j] = dr[j];
+          }
+        }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           sc = E::mfma(at_lane.rows(qt, 0, kk), k[kk], sc);
@@ -637,16 +712,9 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
         }
         float p[16], ds[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int r = 8 * g + 4 * (lane >> 5);
-          const float4v ls = *reinterpret_cast<const float4v*>(st + r);
-          const float4v dr = *reinterpret_cast<const float4v*>(st + QT + r);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = 4 * g + j;
-            p[i] = exp2_of(sc[i] * sl2 - ls[j]);
-            ds[i] = p[i] * (dp[i] * a.scale - dr[j]);
-          }
+        for (int i = 0; i < 16; ++i) {
+          p[i] = exp2_of(sc[i] * sl2);
+          ds[i] = p[i] * (dp[i] * a.scale);
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -657,6 +725,10 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
             dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sb, dk[f]);
           }
         }
+        // reads stay four fragments ahead of the products
+        sched_reads<8>();
+        order<4 * (DP / 32) - 4, 2, 0>();
+        sched_mfma<4>();
       }
       __syncthreads();
     };
@@ -738,6 +810,7 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
               "attn_packed: D must be a multiple of 8, at most 128");
   TORCH_CHECK(rows_aligned(q) && rows_aligned(k) && rows_aligned(v),
               "attn_packed: rows must be dense and 16-byte aligned");
+  TORCH_CHECK(scale > 1e-30 && scale < 1e30, "attn_packed: scale must be positive");
   TORCH_CHECK(q.size(0) < (1L << 30), "attn_packed: too many rows");
   TORCH_CHECK(cu.dim() == 1 && cu.size(0) >= 2 && cu.is_contiguous() &&
               cu.scalar_type() == torch::kInt,
@@ -799,7 +872,7 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
 
 }  // namespace
 
-// {o [T,H,D], lse [H,T] in units of log 2, +inf for rows without tokens}
+// {o [T,H,D], lse [H,T]: -log sum exp(s) / scale, -inf for rows without tokens}
 std::vector<torch::Tensor> attn_packed_fwd(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu,
     c10::optional<torch::Tensor> lengths, bool causal, int64_t window,

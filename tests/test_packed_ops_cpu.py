@@ -59,7 +59,10 @@ def test_attention_refuses():
             ((q, k, k, cu), {"lengths": torch.tensor([6])}),
             ((q, k, k, cu), {"window": 4}),
             ((q, k, k, cu), {"window": 0, "causal": True}),
-            ((q, k, k, cu), {"scale": math.inf})):
+            ((q, k, k, cu), {"scale": math.inf}),
+            ((q, k, k, cu), {"scale": 0.0}),
+            ((q, k, k, cu), {"scale": -0.1}),
+            ((q, k, k, cu), {"scale": math.nan})):
         with pytest.raises(ValueError, match="flash_attention_packed"):
             flash_attention_packed(*args, **kw)
 
