@@ -112,12 +112,19 @@ struct RopeAxes : Function<RopeAxes> {
   }
 };
 
+// The gate as [G, D]: inside of the function, where a view costs no node.
+OptTensor gate_rows(const OptTensor& gate, const Tensor& h) {
+  if (!gate) return gate;
+  return gate->contiguous().view({gate->numel() / h.size(-1), h.size(-1)});
+}
+
 struct BlockNorm : Function<BlockNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& h,
                                const Tensor& x, const Tensor& w1,
                                const Tensor& w2, const OptTensor& gate,
                                double alpha, double eps) {
-    auto r = block_norm_fwd(h, x, w1, w2, gate, alpha, eps, true);
+    auto r = block_norm_fwd(h, x, w1, w2, gate_rows(gate, h), alpha, eps,
+                            true);
     // the sum is computed again in backward, from h and x
     ctx->save_for_backward({h, x, w1, w2, gate.value_or(Tensor()), r[2],
                             r[3]});
@@ -127,9 +134,9 @@ struct BlockNorm : Function<BlockNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto s = ctx->get_saved_variables();
     auto g = block_norm_bwd(grad[0].contiguous(), grad[1].contiguous(), s[0],
-                            s[1], s[2], s[3], maybe(s[4]), s[5], s[6],
-                            ctx->saved_data["alpha"].toDouble());
-    if (!s[4].defined()) g[4] = Tensor();
+                            s[1], s[2], s[3], gate_rows(maybe(s[4]), s[0]),
+                            s[5], s[6], ctx->saved_data["alpha"].toDouble());
+    g[4] = s[4].defined() ? g[4].view(s[4].sizes()) : Tensor();
     g = once(std::move(g), "fused_block_norm");
     return {g[0], g[1], g[2], g[3], g[4], Tensor(), Tensor()};
   }
@@ -168,10 +175,10 @@ std::vector<Tensor> block_norm(Tensor h, Tensor x, Tensor w1, Tensor w2,
   x = x.contiguous();
   w1 = w1.contiguous();
   w2 = w2.contiguous();
-  if (gate) gate = gate->reshape({-1, h.size(-1)}).contiguous();
   const Tensor none;
   if (!wants_grad({&h, &x, &w1, &w2, gate ? &*gate : &none})) {
-    auto r = block_norm_fwd(h, x, w1, w2, gate, alpha, eps, false);
+    auto r = block_norm_fwd(h, x, w1, w2, gate_rows(gate, h), alpha, eps,
+                            false);
     return {r[0], r[1]};
   }
   return BlockNorm::apply(h, x, w1, w2, gate, alpha, eps);
