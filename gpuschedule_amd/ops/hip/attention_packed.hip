@@ -605,9 +605,9 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 
 // ---- backward: dK and dV -----------------------------------------------
 // A block owns 128 keys of one kv head and goes through the query tiles of
-// `rep / splits` of its heads.  Where kv heads and tiles are too few to fill
-// the card, the heads are split among blocks, which leave their sums in
-// fp32, and one more kernel adds those in a fixed order.
+// all its heads.  Where kv heads and key tiles are too few to fill the card,
+// or to even out their lengths, the query tiles are split among blocks, which
+// leave their sums in fp32, and one more kernel adds those in a fixed order.
 //
 // Registers are what this kernel is short of: two accumulators of 32 x DP
 // and a fragment of k take 160 of the 256 that two waves on a SIMD leave, so
@@ -627,14 +627,13 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) float s1[2 * QT];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rep = a.H / a.HK, mine = rep / a.splits;
+  const int rep = a.H / a.HK;
   Lane<DP> at_lane(lane);
   int vh, slot, none, row0;
   Seq s;
   if (!unit_of(a, a.HK * a.splits, 1, false, vh, slot, none)) return;
   if (!tile_of<OWN>(a, slot, s, row0)) return;
   const int kvh = vh / a.splits, split = vh % a.splits;
-  const int h0 = kvh * rep + split * mine;
   const int first = row0 + wave * 32, key = first + (lane & 31);
   const bool live = key < s.len;
   const long at = s.begin + key;
@@ -672,7 +671,12 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
             (__attribute__((address_space(3))) unsigned*)st, 4, 0, 0);
       }
     };
-    int head = h0, t = t1 - 1;
+    // Of all query tiles of all heads this block takes its share.  From the
+    // last tile down: blocks of one head begin at the same ones.
+    const long tiles = t1 - t0, all = rep * tiles;
+    long n = all * split / a.splits;
+    const long stop = all * (split + 1) / a.splits;
+    int head = kvh * rep + (int)(n / tiles), t = t1 - 1 - (int)(n % tiles);
     auto tile = [&](const char* qt, const char* dt, const float* st, char* qn,
                     char* dn, float* sn) __attribute__((always_inline)) {
       const int r0 = t * QT;
@@ -681,7 +685,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
         t = t1 - 1;
         ++head;
       }
-      if (head < h0 + mine) fetch(head, t, qn, dn, sn);
+      if (++n < stop) fetch(head, t, qn, dn, sn);
       if ((!CAUSAL || r0 + QT > first) && first < s.len &&
           (!a.window || r0 <= last + a.window - 1)) {
         float16v sc, dp;           // begin as -lse and -D of their rows
@@ -732,11 +736,11 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
       }
       __syncthreads();
     };
-    fetch(head, t, q0, d0, s0);
+    if (n < stop) fetch(head, t, q0, d0, s0);
     __syncthreads();
-    while (head < h0 + mine) {
+    while (n < stop) {
       tile(q0, d0, s0, q1, d1, s1);
-      if (head < h0 + mine) tile(q1, d1, s1, q0, d0, s0);
+      if (n < stop) tile(q1, d1, s1, q0, d0, s0);
     }
   }
   if (key >= s.rows) return;
@@ -924,12 +928,17 @@ std::vector<torch::Tensor> attn_packed_bwd(
   auto stream = c10::cuda::getCurrentCUDAStream();
   const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
   PACKED_LAUNCH(packed_bwd_q_kernel, a.HK, a.H / a.HK);
-  // two blocks of four waves on each of 256 CUs run at once: twice as many
-  // blocks even out their lengths
-  const int rep = a.H / a.HK;
-  while (a.splits < rep && (long)a.slots * a.HK * a.splits < 1024) {
-    do ++a.splits; while (rep % a.splits);
-  }
+  // Two blocks of four waves on each of 256 CUs run at once: about twice as
+  // many even out their lengths, but a block should keep eight query tiles
+  // (of sequences of the mean length).  One document of 8192 tokens, 16 and
+  // 4 heads of 128: 1656 us for the backward pass unsplit (260 blocks), 1113
+  // in two, 934 in four; documents of 900 tokens, 32 and 8 heads: 711 unsplit
+  // (592 blocks), 528 in two, 568 in four.
+  const long units = (long)a.slots * a.HK;
+  long seen = a.T / a.B + 1;
+  if (a.window) seen = std::min<long>(seen, a.window + OWN);
+  const long most = std::max<long>(1, seen / QT * (a.H / a.HK) / 8);
+  a.splits = (int)std::min({(1023 + units) / units, most, 16L});
   torch::Tensor part;
   if (a.splits > 1) {
     part = torch::empty({a.splits, 2, a.T, a.HK, a.D}, lse.options());
