@@ -26,7 +26,10 @@ def _with_grad(parameters):
 
 def _cpu_grads(params) -> List[torch.Tensor]:
     # a tied weight counts once
-    return [p.grad for p in dict.fromkeys(params) if p.grad is not None]
+    grads = [p.grad for p in dict.fromkeys(params) if p.grad is not None]
+    if any(g.device.type != "cpu" for g in grads):
+        raise RuntimeError("grad_norm: all gradients must be on one device")
+    return grads
 
 
 def _cpu_norm(grads) -> torch.Tensor:

@@ -50,7 +50,8 @@ def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
     through.  1 to 4 axes; q and k both bf16, fp16 or fp32.
 
     Returns new contiguous ``(q, k)``.  A position outside of the tables
-    makes that token's values on that axis NaN."""
+    makes that token's values on that axis NaN.  The tables get no
+    gradient."""
     sections = [int(n) for n in sections]
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] \
             or q.shape[2] != k.shape[2]:
@@ -82,6 +83,7 @@ def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
     if q.is_cuda:
         return tuple(get_ext(required=True).rope_axes(
             q, k, positions, cosb, sinb, sections))
+    cosb, sinb = cosb.detach(), sinb.detach()
     axis = torch.repeat_interleave(torch.arange(len(sections)),
                                    torch.tensor(sections))
     at = positions[axis].t().long()                        # [T, R/2]

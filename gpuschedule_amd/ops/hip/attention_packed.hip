@@ -791,10 +791,19 @@ __global__ __launch_bounds__(NTH) void packed_bwd_sum_kernel(
 
 // ---- host --------------------------------------------------------------
 
-bool rows_aligned(const torch::Tensor& t) {
-  return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-         t.stride(0) < (1 << 24) && (size_t)t.data_ptr() % 16 == 0;
+}  // namespace
+
+// Whether 16-byte reads can follow the strides of t [T, heads, D] (that of a
+// dimension of one is never used).
+bool attn_rows_aligned(const torch::Tensor& t) {
+  return t.stride(2) == 1 &&
+         (t.size(0) == 1 ||
+          (t.stride(0) % 8 == 0 && t.stride(0) < (1 << 24))) &&
+         (t.size(1) == 1 || t.stride(1) % 8 == 0) &&
+         (size_t)t.data_ptr() % 16 == 0;
 }
+
+namespace {
 
 Args args_of(const torch::Tensor& q, const torch::Tensor& k,
              const torch::Tensor& v, const torch::Tensor& cu,
@@ -812,7 +821,7 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
               "attn_packed: kv heads must divide q heads");
   TORCH_CHECK(q.size(2) % 8 == 0 && q.size(2) >= 8 && q.size(2) <= 128,
               "attn_packed: D must be a multiple of 8, at most 128");
-  TORCH_CHECK(rows_aligned(q) && rows_aligned(k) && rows_aligned(v),
+  TORCH_CHECK(attn_rows_aligned(q) && attn_rows_aligned(k) && attn_rows_aligned(v),
               "attn_packed: rows must be dense and 16-byte aligned");
   TORCH_CHECK(scale > 1e-30 && scale < 1e30, "attn_packed: scale must be positive");
   TORCH_CHECK(q.size(0) < (1L << 30), "attn_packed: too many rows");
@@ -906,7 +915,7 @@ std::vector<torch::Tensor> attn_packed_bwd(
   Args a = args_of(q, k, v, cu, lengths, window, scale);
   TORCH_CHECK(dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&
               o.is_contiguous() && dout.scalar_type() == q.scalar_type() &&
-              o.scalar_type() == q.scalar_type() && rows_aligned(dout) &&
+              o.scalar_type() == q.scalar_type() && attn_rows_aligned(dout) &&
               dout.device() == q.device(),
               "attn_packed: o and dout must be like q, dout's rows dense and "
               "16-byte aligned");

@@ -17,6 +17,7 @@ std::vector<Tensor> attn_packed_bwd(Tensor q, Tensor k, Tensor v, Tensor o,
                                     Tensor dout, Tensor lse, Tensor cu,
                                     OptTensor lengths, bool causal,
                                     int64_t window, double scale);
+bool attn_rows_aligned(const Tensor& t);
 std::vector<Tensor> rope_axes(Tensor q, Tensor k, Tensor pos, Tensor cosb,
                               Tensor sinb, std::vector<int64_t> sections,
                               bool backward);
@@ -55,13 +56,9 @@ variable_list once(variable_list grads, const char* what) {
 // t, or a copy of it where 16-byte reads cannot follow its strides (an
 // expanded gradient, whose strides are 0, is read as it is)
 Tensor aligned_rows(const Tensor& t) {
-  auto ok = [](const Tensor& x) {
-    return x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 &&
-           x.stride(0) < (1 << 24) && (size_t)x.data_ptr() % 16 == 0;
-  };
-  if (ok(t)) return t;
+  if (attn_rows_aligned(t)) return t;
   auto c = t.contiguous();
-  return ok(c) ? c : c.clone();
+  return attn_rows_aligned(c) ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 
 Tensor dense_rows(const Tensor& t) {
@@ -162,8 +159,8 @@ std::vector<Tensor> rope_axes_grad(Tensor q, Tensor k, Tensor pos,
   q = dense_rows(q);
   k = dense_rows(k);
   pos = pos.contiguous();
-  cosb = cosb.contiguous();
-  sinb = sinb.contiguous();
+  cosb = cosb.detach().contiguous();
+  sinb = sinb.detach().contiguous();
   if (!wants_grad({&q, &k}))
     return rope_axes(q, k, pos, cosb, sinb, sections, false);
   return RopeAxes::apply(q, k, pos, cosb, sinb, sections);

@@ -144,7 +144,7 @@ def fused_block_norm(h: torch.Tensor, x: torch.Tensor,
         raise ValueError(f"fused_block_norm: bf16, fp16 or fp32 only, "
                          f"got {h.dtype}")
     if gate is not None and gate.shape != (D,) and gate.shape != h.shape \
-            and gate.shape != (h.shape[0], D):
+            and (h.dim() < 2 or gate.shape != (h.shape[0], D)):
         raise ValueError(f"fused_block_norm: gate {tuple(gate.shape)} is "
                          f"none of [D], [h.shape[0], D] and h's shape")
     if not h.is_cuda:

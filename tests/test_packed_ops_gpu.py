@@ -271,6 +271,24 @@ def test_attention_layouts():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_attention_one_row_of_any_stride():
+    """The stride of a dimension of one says nothing."""
+    room = normal((4, 1, 2 * 64 + 1), BF, 3)
+    q = room[:1, :, :64]
+    assert q.stride(0) % 8
+    k = room.as_strided((1, 1, 64), (129, 5, 1), 64)
+    leaves = [t.detach().requires_grad_() for t in (q, k, k)]
+    o = flash_attention_packed(*leaves, cu_of([1]))
+    assert torch.equal(o, k)                 # one key: its value
+    dq, dk, dv = torch.autograd.grad(o, leaves, o)
+    assert torch.equal(dv, o)
+    # p (dP - D) is 0; both sums of 64 products are off by at most 64 2^-24 of
+    # their terms, and p by 2^-20
+    off = 2.0 ** -14 / 8 * (o.double() * k.double()).abs().sum()
+    assert (dq.double().abs() <= off * k.double().abs()).all()
+    assert (dk.double().abs() <= off * q.double().abs()).all()
+
+
 def test_attention_is_the_same_every_time():
     q, k, v = qkv_of(2000, 8, 2, 128, BF, 21)
     do = normal((2000, 8, 128), BF, 22)
@@ -406,6 +424,16 @@ def test_rope_far_and_bad_positions():
     y = y.unflatten(-1, (2, 32))
     assert y[1:, :, :, :8].isnan().all()      # those tokens, that axis
     assert not y[0].isnan().any() and not y[..., 8:].isnan().any()
+
+
+def test_rope_tables_get_no_gradient():
+    cos, sin = rope_tables(9, 16)
+    cos.requires_grad_()
+    pos = torch.zeros(1, 5, dtype=torch.int64, device="cuda")
+    q, k, _ = qkv_of(5, 3, 1, 40, BF, 3)
+    out, _ = fused_rope_axes(q, k, pos, cos, sin, [16])
+    out.sum().backward()
+    assert cos.grad is None and q.grad is not None
 
 
 def test_rope_odd_gradients_and_nothing():
@@ -836,10 +864,29 @@ def test_refusals_on_the_device():
     d.grad = torch.zeros_like(d)
     with pytest.raises(RuntimeError, match="bf16, fp16 or fp32"):
         clip_grad_norm_([d], 1.0)
+    one = torch.ones(64, device="cuda", dtype=BF)
+    with pytest.raises(ValueError, match="gate"):
+        fused_block_norm(one, one, w, w, torch.ones(64, 64, device="cuda",
+                                                    dtype=BF))
+    d.grad = None
+    p[0].grad = torch.zeros(8, device="cuda")
+    p[1].grad = None
+    host = torch.nn.Parameter(torch.zeros(3))
+    host.grad = torch.zeros(3)
+    for both in ([p[0], host], [host, p[0]]):
+        with pytest.raises(RuntimeError, match="one"):
+            clip_grad_norm_(both, 1.0)
     # a second derivative is refused, not wrong
     x = torch.ones(2, 8, device="cuda", requires_grad=True)
     v = torch.ones(8, device="cuda", requires_grad=True)
     n, _ = fused_block_norm(x, x, v, v)
     (g,) = torch.autograd.grad(n.sum(), v, create_graph=True)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(RuntimeError, match="second derivative"):
         g.sum().backward()
+    q = normal((8, 2, 64), BF, 1).requires_grad_()
+    for out in (flash_attention_packed(q, q, q, cu),
+                fused_rope_axes(q, q, pos, cos, sin, [32])[0]):
+        (g,) = torch.autograd.grad(out.float().square().sum(), q,
+                                   create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            g.float().sum().backward()
