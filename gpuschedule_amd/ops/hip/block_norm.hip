@@ -59,16 +59,58 @@ template <class T> __device__ __forceinline__ float part_of(uint4v w, int j) {
   }
 }
 
+// w without its first `bytes` (1 to 15), zeros at its end.
+__device__ __forceinline__ uint4v shifted(uint4v w, int bytes) {
+  unsigned long lo = (unsigned long)w[1] << 32 | w[0];
+  unsigned long hi = (unsigned long)w[3] << 32 | w[2];
+  const int s = bytes * 8;
+  lo = s < 64 ? lo >> s | hi << (64 - s) : hi >> (s - 64);
+  hi = s < 64 ? hi >> s : 0;
+  return uint4v{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi,
+                (unsigned)(hi >> 32)};
+}
+
 template <class T> __device__ __forceinline__ unsigned bits_of(T v) {
   if constexpr (sizeof(T) == 4) return __builtin_bit_cast(unsigned, v);
   else return __builtin_bit_cast(unsigned short, v);
+}
+
+// w with v put before its first value.
+template <class T> __device__ __forceinline__ uint4v pushed(uint4v w, T v) {
+  if constexpr (sizeof(T) == 4) return uint4v{bits_of(v), w[0], w[1], w[2]};
+  else return uint4v{w[0] << 16 | bits_of(v), w[1] << 16 | w[0] >> 16,
+                     w[2] << 16 | w[1] >> 16, w[3] << 16 | w[2] >> 16};
+}
+
+// Writes the first n values of w (n less than a run's).
+template <class T>
+__device__ __forceinline__ void store_part(T* p, uint4v w, int n) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Two { unsigned a, b; };
+  struct __attribute__((packed, aligned(sizeof(T)))) One { unsigned a; };
+  constexpr int PER = 4 / sizeof(T);       // values of a register
+  if (n & 2 * PER) {
+    *reinterpret_cast<Two*>(p) = Two{w[0], w[1]};
+    p += 2 * PER;
+    w[0] = w[2];
+    w[1] = w[3];
+  }
+  if (n & PER) {
+    *reinterpret_cast<One*>(p) = One{w[0]};
+    p += PER;
+    w[0] = w[1];
+  }
+  if constexpr (PER == 2) {
+    const unsigned short last = (unsigned short)w[0];
+    if (n & 1) *p = __builtin_bit_cast(T, last);
+  }
 }
 
 // The part of a row that a thread holds: E values as runs of 16 bytes, ROWT
 // threads side by side, kept as they were read until they are used.  EVEN:
 // D is a multiple of a run, so that no run ends inside of it.  Without the
 // code for that, 16384 rows of 4096 bf16 take 95 and 170 us forward and
-// backward; with it 102 and 176.
+// backward; with it 102 and 176.  Rows whose width is odd begin off the lines
+// of memory, too: 12474 rows of 1440 fp16 take 24 us forward, of 1435 40.
 template <class T, int ROWT, int E, bool EVEN> struct Row {
   static constexpr int V = WIDE<T>, C = E / V;
   uint4v r[C];
@@ -86,12 +128,13 @@ template <class T, int ROWT, int E, bool EVEN> struct Row {
       } else if (i + V <= D) {
         r[c] = reinterpret_cast<const Run<T>*>(p + i)->w;
       } else {
-        constexpr int PER = 4 / sizeof(T);   // values of a register
         r[c] = (uint4v)(0);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (i + j < D)
-            r[c][j / PER] |= bits_of(p[i + j]) << (j % PER * 16);
+        if (i < D && D >= V)       // the row's last run, less what is not ours
+          r[c] = shifted(reinterpret_cast<const Run<T>*>(p + D - V)->w,
+                         (i + V - D) * (int)sizeof(T));
+        else if (i < D)
+          for (int j = D - i - 1; j >= 0; --j)
+            r[c] = pushed<T>(r[c], p[i + j]);
       }
     }
   }
@@ -109,18 +152,15 @@ template <class T, int ROWT, int E, bool EVEN> struct Row {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = at(t, c);
-      if (EVEN ? i < D : i + V <= D) {
-        constexpr int PER = 4 / sizeof(T);
-        Run<T> w = {(uint4v)(0)};
+      constexpr int PER = 4 / sizeof(T);
+      Run<T> w = {(uint4v)(0)};
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          w.w[j / PER] |= bits_of(down<T>(v[c * V + j])) << (j % PER * 16);
+      for (int j = 0; j < V; ++j)
+        w.w[j / PER] |= bits_of(down<T>(v[c * V + j])) << (j % PER * 16);
+      if (EVEN ? i < D : i + V <= D)
         *reinterpret_cast<Run<T>*>(p + i) = w;
-      } else if (!EVEN) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (i + j < D) p[i + j] = down<T>(v[c * V + j]);
-      }
+      else if (!EVEN && i < D)
+        store_part(p + i, w.w, D - i);
     }
   }
   static __device__ __forceinline__ void store32(float* p, int D, int t,
@@ -244,8 +284,12 @@ __device__ __forceinline__ void block_add(float (&v)[E], float* room) {
 // and finishes their rows of dg.  Otherwise `slices` blocks share a group of
 // rows, `per` rows each, which the workers take in turn, and sum(e hh) of
 // the group is left in parts too.
+// 16-bit rows fit four waves on a SIMD (128 registers); 32-bit ones spill
+// there, and are faster with three: 12474 rows of 1024, a gate for each, 169
+// us forward and backward with four, 144 with three.
 template <class T, int ROWT, int E, bool EVEN, bool WHOLE>
-__global__ __launch_bounds__(BLOCK<ROWT>, 4) void block_norm_bwd_kernel(
+__global__ __launch_bounds__(BLOCK<ROWT>, sizeof(T) == 2 || ROWT > 256 ? 4 : 3)
+void block_norm_bwd_kernel(
     const T* __restrict__ dn, const T* __restrict__ ds,
     const T* __restrict__ h, const T* __restrict__ x,
     const T* __restrict__ w1, const T* __restrict__ w2,
