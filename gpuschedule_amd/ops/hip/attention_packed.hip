@@ -76,7 +76,6 @@ struct FH {
   }
 };
 
-
 constexpr int NW = 4, NTH = NW * 64;
 constexpr int TILE = 64;           // rows of a staged tile
 constexpr int OWN = 32 * NW;       // rows that a block owns: 32 a wave
@@ -522,7 +521,10 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     // D = dO.o carries the rounding of o, and of the probabilities that went
     // into it: next to nothing where many keys share a row, but with few it
     // is half of the error of dQ and dK.  Where a block's rows see no more
-    // keys than its two buffers hold, D is the sum of p dP instead.
+    // keys than its two buffers hold, D is the sum of p dP instead (32 rows
+    // of 128 tokens, 12 heads of 64: 16.5 us for 13.2; with sequences of 20
+    // tokens dQ and dK are off by 1.4 times what rounding their exact values
+    // costs, else by 1.8).
     const bool few = t1 - t <= 2;
     auto dots = [&](int t, const char* kt, const char* vt)
         __attribute__((always_inline)) {
@@ -749,7 +751,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
     put_rows<E, DP>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dv);
   } else {
     const long n = (long)a.T * a.HK * a.D;
-    float* p = a.part + (2 * split * a.T + at) * a.HK * a.D + kvh * a.D;
+    float* p = a.part + (2L * split * a.T + at) * a.HK * a.D + kvh * a.D;
 #pragma unroll
     for (int f = 0; f < DP / 32; ++f)
 #pragma unroll
@@ -824,7 +826,7 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   TORCH_CHECK(attn_rows_aligned(q) && attn_rows_aligned(k) && attn_rows_aligned(v),
               "attn_packed: rows must be dense and 16-byte aligned");
   TORCH_CHECK(scale > 1e-30 && scale < 1e30, "attn_packed: scale must be positive");
-  TORCH_CHECK(q.size(0) < (1L << 30), "attn_packed: too many rows");
+  TORCH_CHECK(q.size(0) < (1L << 29), "attn_packed: too many rows");
   TORCH_CHECK(cu.dim() == 1 && cu.size(0) >= 2 && cu.is_contiguous() &&
               cu.scalar_type() == torch::kInt,
               "attn_packed: cu_seqlens must be int32 [sequences + 1]");
