@@ -30,6 +30,9 @@ std::vector<Tensor> block_norm_bwd(Tensor dn, Tensor ds, Tensor h, Tensor x,
 
 namespace {
 
+// Allocations and views inside of a function need no trace of their own.
+using Untraced = at::AutoDispatchBelowADInplaceOrView;
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const auto* t : ts)
@@ -70,6 +73,7 @@ struct PackedAttn : Function<PackedAttn> {
                         const Tensor& v, const Tensor& cu,
                         const OptTensor& lengths, bool causal, int64_t window,
                         double scale) {
+    Untraced untraced;
     auto r = attn_packed_fwd(q, k, v, cu, lengths, causal, window, scale);
     ctx->save_for_backward({q, k, v, r[0], r[1], cu,
                             lengths.value_or(Tensor())});
@@ -80,11 +84,15 @@ struct PackedAttn : Function<PackedAttn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto s = ctx->get_saved_variables();
-    auto g = attn_packed_bwd(s[0], s[1], s[2], s[3], aligned_rows(grad[0]),
-                             s[4], s[5], maybe(s[6]),
-                             ctx->saved_data["causal"].toBool(),
-                             ctx->saved_data["window"].toInt(),
-                             ctx->saved_data["scale"].toDouble());
+    variable_list g;
+    {
+      Untraced untraced;
+      g = attn_packed_bwd(s[0], s[1], s[2], s[3], aligned_rows(grad[0]), s[4],
+                          s[5], maybe(s[6]),
+                          ctx->saved_data["causal"].toBool(),
+                          ctx->saved_data["window"].toInt(),
+                          ctx->saved_data["scale"].toDouble());
+    }
     g = once(std::move(g), "flash_attention_packed");
     return {g[0], g[1], g[2], Tensor(), Tensor(), Tensor(), Tensor(),
             Tensor()};
@@ -98,12 +106,17 @@ struct RopeAxes : Function<RopeAxes> {
                                std::vector<int64_t> sections) {
     ctx->save_for_backward({pos, cosb, sinb});
     ctx->saved_data["sections"] = sections;
+    Untraced untraced;
     return rope_axes(q, k, pos, cosb, sinb, sections, false);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto s = ctx->get_saved_variables();
-    auto g = rope_axes(dense_rows(grad[0]), dense_rows(grad[1]), s[0], s[1],
-                       s[2], ctx->saved_data["sections"].toIntVector(), true);
+    variable_list g;
+    {
+      Untraced untraced;
+      g = rope_axes(dense_rows(grad[0]), dense_rows(grad[1]), s[0], s[1], s[2],
+                    ctx->saved_data["sections"].toIntVector(), true);
+    }
     g = once(std::move(g), "fused_rope_axes");
     return {g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -120,6 +133,7 @@ struct BlockNorm : Function<BlockNorm> {
                                const Tensor& x, const Tensor& w1,
                                const Tensor& w2, const OptTensor& gate,
                                double alpha, double eps) {
+    Untraced untraced;
     auto r = block_norm_fwd(h, x, w1, w2, gate_rows(gate, h), alpha, eps,
                             true);
     // the sum is computed again in backward, from h and x
@@ -130,10 +144,14 @@ struct BlockNorm : Function<BlockNorm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto s = ctx->get_saved_variables();
-    auto g = block_norm_bwd(grad[0].contiguous(), grad[1].contiguous(), s[0],
-                            s[1], s[2], s[3], gate_rows(maybe(s[4]), s[0]),
-                            s[5], s[6], ctx->saved_data["alpha"].toDouble());
-    g[4] = s[4].defined() ? g[4].view(s[4].sizes()) : Tensor();
+    variable_list g;
+    {
+      Untraced untraced;
+      g = block_norm_bwd(grad[0].contiguous(), grad[1].contiguous(), s[0],
+                         s[1], s[2], s[3], gate_rows(maybe(s[4]), s[0]), s[5],
+                         s[6], ctx->saved_data["alpha"].toDouble());
+      g[4] = s[4].defined() ? g[4].view(s[4].sizes()) : Tensor();
+    }
     g = once(std::move(g), "fused_block_norm");
     return {g[0], g[1], g[2], g[3], g[4], Tensor(), Tensor()};
   }
