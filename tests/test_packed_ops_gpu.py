@@ -313,6 +313,25 @@ def test_attention_bad_cu_stays_inside():
     assert all(torch.isfinite(t).all() for t in (q, k, v))
 
 
+def test_attention_offsets_past_32_bits():
+    """q has over 2^31 values; the last sequence lies behind them."""
+    T, n, H, HK, D = 270_000, 300, 64, 2, 128
+    assert (T - n) * H * D > 1 << 31
+    q, do = (torch.zeros(T, H, D, device="cuda", dtype=BF) for _ in range(2))
+    k, v = (torch.zeros(T, HK, D, device="cuda", dtype=BF) for _ in range(2))
+    for i, t in enumerate((q, k, v, do)):
+        t[-n:] = normal((n,) + t.shape[1:], BF, 60 + i)
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    o = flash_attention_packed(q, k, v, cu_of([T - n, n]), causal=True,
+                               window=64)
+    got = (o,) + torch.autograd.grad(o, (q, k, v), do)
+    seen = seen_of([n], None, n, True, 64)
+    want = oracle(*(t.detach()[-n:] for t in (q, k, v, do)), seen, D ** -0.5)
+    for g, (w, tol), name in zip(got, want, ("o", "dq", "dk", "dv")):
+        within(g[-n:], w, tol, name)
+        assert (g[:-n] == 0).all()
+
+
 def test_attention_agrees_with_differences():
     """The gradients along a direction against differences of the 64-bit
     forward pass (h^2 error about 1e-6 of the second derivative)."""
@@ -434,6 +453,23 @@ def test_rope_tables_get_no_gradient():
     out, _ = fused_rope_axes(q, k, pos, cos, sin, [16])
     out.sum().backward()
     assert cos.grad is None and q.grad is not None
+
+
+def test_rope_more_tokens_than_one_row_of_blocks():
+    T = (1 << 29) + 77
+    q, k = (torch.ones(T, 1, 2, device="cuda", dtype=BF) for _ in range(2))
+    cos, sin = rope_tables(4, 1)
+    pos = torch.zeros(1, T, device="cuda", dtype=torch.int32)
+    at = [0, 1 << 28, (1 << 29) - 1, 1 << 29, T - 1]
+    pos[0, at] = torch.tensor([1, 2, 3, 1, 2], device="cuda",
+                              dtype=torch.int32)
+    for y in fused_rope_axes(q, k, pos, cos, sin, [1]):
+        for i, p in zip(at, (1, 2, 3, 1, 2)):
+            c, s = cos[p, 0].double(), sin[p, 0].double()
+            want = torch.stack([c - s, c + s])[None]
+            within(y[i], want, unit(BF) * want.abs() + 2.0 ** -22, "turned")
+        y[at] = 1
+        assert (y == 1).all()
 
 
 def test_rope_odd_gradients_and_nothing():
@@ -568,6 +604,25 @@ def test_block_norm_layouts_and_parts():
     n, s = fused_block_norm(z, z, v, v)
     (dv,) = torch.autograd.grad(n.sum() + s.sum(), v)
     assert (dv == 0).all()
+
+
+def test_block_norm_offsets_past_32_bits():
+    """Rows behind 2^31 values come out as by themselves."""
+    rows, D, n = 530_000, 4096, 5
+    assert (rows - n) * D > 1 << 31
+    tail = [normal((n, D), BF, i) for i in range(4)]
+    h, x, dn, ds = (torch.zeros(rows, D, device="cuda", dtype=BF)
+                    for _ in range(4))
+    for t, e in zip((h, x, dn, ds), tail):
+        t[-n:] = e
+    w = normal((D,), BF, 9, 0.2, 1)
+    out = []
+    for a, b, c, d in ((h, x, dn, ds), tail):
+        a, b = a.requires_grad_(), b.requires_grad_()
+        got = fused_block_norm(a, b, w, w, w)
+        out.append(got + torch.autograd.grad(got, (a, b), (c, d)))
+    for big, small in zip(*out):
+        assert torch.equal(big[-n:], small) and (big[:-n] == 0).all()
 
 
 def test_block_norm_agrees_with_differences():
