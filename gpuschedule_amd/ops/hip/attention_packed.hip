@@ -240,24 +240,24 @@ template <int DP> struct Lane {
   }
 };
 
-// B operand straight from global memory: row of this lane, DP / 16 steps.
-template <int DP>
+// B operand straight from global memory: row of this lane, DC / 16 steps.
+template <int DC>
 __device__ __forceinline__ void own_rows(const short* p, bool ok, int D,
-                                         int lane, short8 (&v)[DP / 16]) {
+                                         int lane, short8 (&v)[DC / 16]) {
 #pragma unroll
-  for (int kk = 0; kk < DP / 16; ++kk) {
+  for (int kk = 0; kk < DC / 16; ++kk) {
     const int d = 16 * kk + 8 * (lane >> 5);
     v[kk] = ok && d < D ? *reinterpret_cast<const short8*>(p + d)
                         : short8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
 
-// The accumulator of a [DP][32 rows] product: lane's row gets its values.
-template <class E, int DP>
+// The accumulator of a [DC][32 rows] product: lane's row gets its values.
+template <class E, int DC>
 __device__ __forceinline__ void put_rows(short* p, bool live, int D, int lane,
-                                         float by, const float16v (&acc)[DP / 32]) {
+                                         float by, const float16v (&acc)[DC / 32]) {
 #pragma unroll
-  for (int f = 0; f < DP / 32; ++f)
+  for (int f = 0; f < DC / 32; ++f)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * f + 8 * g + 4 * (lane >> 5);
@@ -330,8 +330,9 @@ __device__ __forceinline__ bool seen(const Args& a, int key, int row,
 }
 
 // ---- forward -----------------------------------------------------------
+// DP: values of a row in LDS, DC: those that products take.
 
-template <class E, int DP, bool CAUSAL>
+template <class E, int DP, int DC, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
@@ -352,13 +353,13 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 
   // m: the reference that exponents are taken from, in units of log 2
   float m = kNone, l = 0.f;
-  float16v o[DP / 32];
+  float16v o[DC / 32];
 #pragma unroll
-  for (int f = 0; f < DP / 32; ++f) o[f] = (float16v)(0.f);
+  for (int f = 0; f < DC / 32; ++f) o[f] = (float16v)(0.f);
 
   if (row0 < s.len) {
-    short8 q[DP / 16];
-    own_rows<DP>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
+    short8 q[DC / 16];
+    own_rows<DC>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
     const short* kp = a.k + s.begin * a.k_t + kvh * a.k_h;
     const short* vp = a.v + s.begin * a.v_t + kvh * a.v_h;
     const unsigned koff = stage_offset<DP>(a.k_t);
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
         for (int kb = 0; kb < 2; ++kb) {
           sc[kb] = (float16v)(0.f);
 #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
+          for (int kk = 0; kk < DC / 16; ++kk)
             sc[kb] = E::mfma(at_lane.rows(kt, 32 * kb, kk), q[kk], sc[kb]);
         }
         if (what == 1) {
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           m = mn;
           l *= alpha;
 #pragma unroll
-          for (int f = 0; f < DP / 32; ++f)
+          for (int f = 0; f < DC / 32; ++f)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[f][i] *= alpha;
         }
@@ -432,14 +433,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           // product needs; their sum is taken before
           const short8 pb = E::pack(p);
 #pragma unroll
-          for (int f = 0; f < DP / 32; ++f)
+          for (int f = 0; f < DC / 32; ++f)
             o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pb, o[f]);
         }
         // the first probabilities, then a few more beside each product, whose
         // fragments are read two products ahead
         sched_reads<4>();
         sched_vector<36>();
-        order<DP / 8 - 2, 2, 6>();
+        order<DC / 8 - 2, 2, 6>();
         sched_mfma<2>();
         __builtin_amdgcn_s_setprio(0);
       }
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
   }
   l += other_half(l);
   if (row < s.rows) {
-    put_rows<E, DP>(a.out + (at * a.H + head) * a.D, live, a.D, lane, 1.f / l,
+    put_rows<E, DC>(a.out + (at * a.H + head) * a.D, live, a.D, lane, 1.f / l,
                     o);
     // a row without keys: exp(s - inf) is 0 in backward
     if (lane < 32)
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 
 // ---- backward: dQ, and D for the other kernel --------------------------
 
-template <class E, int DP, bool CAUSAL>
+template <class E, int DP, int DC, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
@@ -485,20 +486,20 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
   const bool live = row < s.len;
   const long at = s.begin + row;
 
-  float16v dq[DP / 32];
+  float16v dq[DC / 32];
 #pragma unroll
-  for (int f = 0; f < DP / 32; ++f) dq[f] = (float16v)(0.f);
+  for (int f = 0; f < DC / 32; ++f) dq[f] = (float16v)(0.f);
 
   if (row0 < s.len) {
-    short8 q[DP / 16], dO[DP / 16];
-    own_rows<DP>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
-    own_rows<DP>(a.dout + at * a.d_t + head * a.d_h, live, a.D, lane, dO);
+    short8 q[DC / 16], dO[DC / 16];
+    own_rows<DC>(a.q + at * a.q_t + head * a.q_h, live, a.D, lane, q);
+    own_rows<DC>(a.dout + at * a.d_t + head * a.d_h, live, a.D, lane, dO);
     float dr = 0.f;
     {
-      short8 ov[DP / 16];
-      own_rows<DP>(a.o + (at * a.H + head) * a.D, live, a.D, lane, ov);
+      short8 ov[DC / 16];
+      own_rows<DC>(a.o + (at * a.H + head) * a.D, live, a.D, lane, ov);
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk)
+      for (int kk = 0; kk < DC / 16; ++kk)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           dr += E::up(ov[kk][j]) * E::up(dO[kk][j]);
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
       for (int kb = 0; kb < 2; ++kb) {
         float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
+        for (int kk = 0; kk < DC / 16; ++kk) {
           sc = E::mfma(at_lane.rows(kt, 32 * kb, kk), q[kk], sc);
           dp = E::mfma(at_lane.rows(vt, 32 * kb, kk), dO[kk], dp);
         }
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
         for (int kb = 0; kb < 2; ++kb) {
           float16v sc = (float16v)(0.f), dp = (float16v)(0.f);
 #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
+          for (int kk = 0; kk < DC / 16; ++kk) {
             sc = E::mfma(at_lane.rows(kt, 32 * kb, kk), q[kk], sc);
             dp = E::mfma(at_lane.rows(vt, 32 * kb, kk), dO[kk], dp);
           }
@@ -577,7 +578,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
           for (int ks = 0; ks < 2; ++ks) {
             const short8 b = E::pack(ds + 8 * ks);
 #pragma unroll
-            for (int f = 0; f < DP / 32; ++f)
+            for (int f = 0; f < DC / 32; ++f)
               dq[f] = E::mfma(at_lane.cols(kt, 32 * kb + 16 * ks, f), b,
                               dq[f]);
           }
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     }
   }
   if (row < s.rows)
-    put_rows<E, DP>(a.dq + (at * a.H + head) * a.D, live, a.D, lane, 1.f, dq);
+    put_rows<E, DC>(a.dq + (at * a.H + head) * a.D, live, a.D, lane, 1.f, dq);
 }
 
 // ---- backward: dK and dV -----------------------------------------------
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 
 constexpr int QT = 32;
 
-template <class E, int DP, bool CAUSAL>
+template <class E, int DP, int DC, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char own_v[OWN * DP * 2];
   __shared__ __attribute__((aligned(16))) char q0[QT * DP * 2];
@@ -640,13 +641,13 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   const bool live = key < s.len;
   const long at = s.begin + key;
 
-  float16v dk[DP / 32], dv[DP / 32];
+  float16v dk[DC / 32], dv[DC / 32];
 #pragma unroll
-  for (int f = 0; f < DP / 32; ++f) dk[f] = dv[f] = (float16v)(0.f);
+  for (int f = 0; f < DC / 32; ++f) dk[f] = dv[f] = (float16v)(0.f);
 
   if (row0 < s.len) {
-    short8 k[DP / 16];
-    own_rows<DP>(a.k + at * a.k_t + kvh * a.k_h, live, a.D, lane, k);
+    short8 k[DC / 16];
+    own_rows<DC>(a.k + at * a.k_t + kvh * a.k_h, live, a.D, lane, k);
     stage<DP, OWN>(a.v + s.begin * a.v_t + kvh * a.v_h, a.v_t,
                    stage_offset<DP>(a.v_t), row0, s.len, a.D, own_v);
     const unsigned qoff = stage_offset<DP>(a.q_t);
@@ -703,7 +704,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
           }
         }
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
+        for (int kk = 0; kk < DC / 16; ++kk) {
           sc = E::mfma(at_lane.rows(qt, 0, kk), k[kk], sc);
           dp = E::mfma(at_lane.rows(dt, 0, kk),
                        at_lane.rows(own_v, wave * 32, kk), dp);
@@ -726,14 +727,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
         for (int ks = 0; ks < 2; ++ks) {
           const short8 pb = E::pack(p + 8 * ks), sb = E::pack(ds + 8 * ks);
 #pragma unroll
-          for (int f = 0; f < DP / 32; ++f) {
+          for (int f = 0; f < DC / 32; ++f) {
             dv[f] = E::mfma(at_lane.cols(dt, 16 * ks, f), pb, dv[f]);
             dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sb, dk[f]);
           }
         }
         // reads stay four fragments ahead of the products
         sched_reads<8>();
-        order<4 * (DP / 32) - 4, 2, 0>();
+        order<4 * (DC / 32) - 4, 2, 0>();
         sched_mfma<4>();
       }
       __syncthreads();
@@ -747,13 +748,13 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   }
   if (key >= s.rows) return;
   if (a.splits == 1) {
-    put_rows<E, DP>(a.dk + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dk);
-    put_rows<E, DP>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dv);
+    put_rows<E, DC>(a.dk + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dk);
+    put_rows<E, DC>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dv);
   } else {
     const long n = (long)a.T * a.HK * a.D;
     float* p = a.part + (2L * split * a.T + at) * a.HK * a.D + kvh * a.D;
 #pragma unroll
-    for (int f = 0; f < DP / 32; ++f)
+    for (int f = 0; f < DC / 32; ++f)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = 32 * f + 8 * g + 4 * (lane >> 5);
@@ -863,26 +864,26 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   return a;
 }
 
+// Rows stand in LDS as 64 or 128 values; of 128, only 96 are computed with
+// where D is no more (8192 tokens, 16 and 4 heads of 80, causal: 262 us
+// forward and 1032 with gradients, with all 128 288 and 1184).
 #define PACKED_LAUNCH(KERNEL, HEADS, REP)                                   \
   do {                                                                      \
-    const dim3 grid((a.slots * (HEADS) + 7) / 8 * 8 * (REP)), block(NTH);   \
-    const auto st = stream.stream();                                        \
-    if (bf && wide && causal)                                               \
-      hipLaunchKernelGGL((KERNEL<BF, 128, true>), grid, block, 0, st, a);   \
-    else if (bf && wide)                                                    \
-      hipLaunchKernelGGL((KERNEL<BF, 128, false>), grid, block, 0, st, a);  \
-    else if (bf && causal)                                                  \
-      hipLaunchKernelGGL((KERNEL<BF, 64, true>), grid, block, 0, st, a);    \
-    else if (bf)                                                            \
-      hipLaunchKernelGGL((KERNEL<BF, 64, false>), grid, block, 0, st, a);   \
-    else if (wide && causal)                                                \
-      hipLaunchKernelGGL((KERNEL<FH, 128, true>), grid, block, 0, st, a);   \
-    else if (wide)                                                          \
-      hipLaunchKernelGGL((KERNEL<FH, 128, false>), grid, block, 0, st, a);  \
-    else if (causal)                                                        \
-      hipLaunchKernelGGL((KERNEL<FH, 64, true>), grid, block, 0, st, a);    \
-    else                                                                    \
-      hipLaunchKernelGGL((KERNEL<FH, 64, false>), grid, block, 0, st, a);   \
+    const dim3 grid((a.slots * (HEADS) + 7) / 8 * 8 * (REP));               \
+    auto launch = [&](auto kernel) {                                        \
+      hipLaunchKernelGGL(kernel, grid, dim3(NTH), 0, stream.stream(), a);   \
+    };                                                                      \
+    auto typed = [&](auto type) {                                           \
+      using E = decltype(type);                                             \
+      if (a.D <= 64 && causal) launch(KERNEL<E, 64, 64, true>);             \
+      else if (a.D <= 64) launch(KERNEL<E, 64, 64, false>);                 \
+      else if (a.D <= 96 && causal) launch(KERNEL<E, 128, 96, true>);       \
+      else if (a.D <= 96) launch(KERNEL<E, 128, 96, false>);                \
+      else if (causal) launch(KERNEL<E, 128, 128, true>);                   \
+      else launch(KERNEL<E, 128, 128, false>);                              \
+    };                                                                      \
+    if (bf) typed(BF());                                                    \
+    else typed(FH());                                                       \
   } while (0)
 
 }  // namespace
@@ -902,7 +903,7 @@ std::vector<torch::Tensor> attn_packed_fwd(
   a.out = (short*)o.data_ptr();
   a.lse = lse.data_ptr<float>();
   auto stream = c10::cuda::getCurrentCUDAStream();
-  const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
+  const bool bf = q.scalar_type() == torch::kBFloat16;
   PACKED_LAUNCH(packed_fwd_kernel, a.HK, a.H / a.HK);
   HIP_CHECK_LAST();
   return {o, lse};
@@ -937,7 +938,7 @@ std::vector<torch::Tensor> attn_packed_bwd(
   a.lse = lse.data_ptr<float>();
   a.drow = drow.data_ptr<float>();
   auto stream = c10::cuda::getCurrentCUDAStream();
-  const bool bf = q.scalar_type() == torch::kBFloat16, wide = a.D > 64;
+  const bool bf = q.scalar_type() == torch::kBFloat16;
   PACKED_LAUNCH(packed_bwd_q_kernel, a.HK, a.H / a.HK);
   // Two blocks of four waves on each of 256 CUs run at once: about twice as
   // many even out their lengths, but a block should keep eight query tiles
