@@ -572,6 +572,14 @@ def test_block_norm_gates(shape, gate):
     check_block_norm(shape, BF, gate, seed=len(shape))
 
 
+@pytest.mark.parametrize("groups,rows", [
+    (350, 5), (700, 3), (1023, 4), (3, 1), (1, 2), (1025, 5), (2050, 5)])
+@pytest.mark.parametrize("D", [512, 1100])
+def test_block_norm_group_counts(groups, rows, D):
+    # about as many groups as blocks: cut, one a block, one a worker, several
+    check_block_norm((groups, rows, D), BF, (groups, D), seed=groups)
+
+
 def test_block_norm_rows_of_zeros_and_scales():
     D = 200
     h = torch.zeros(4, D, device="cuda", dtype=BF)
