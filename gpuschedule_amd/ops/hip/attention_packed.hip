@@ -76,6 +76,15 @@ struct FH {
   }
 };
 
+// What rounding took from 8 values.
+template <class E>
+__device__ __forceinline__ short8 rest(const float* v, short8 rounded) {
+  float w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = v[j] - E::up(rounded[j]);
+  return E::pack(w);
+}
+
 constexpr int NW = 4, NTH = NW * 64;
 constexpr int TILE = 64;           // rows of a staged tile
 constexpr int OWN = 32 * NW;       // rows that a block owns: 32 a wave
@@ -330,9 +339,10 @@ __device__ __forceinline__ bool seen(const Args& a, int key, int row,
 }
 
 // ---- forward -----------------------------------------------------------
-// DP: values of a row in LDS, DC: those that products take.
+// DP: values of a row in LDS, DC: those that products take.  FINE: second
+// factors go in as two values each, rounded and the rest (`is_fine`).
 
-template <class E, int DP, int DC, bool CAUSAL>
+template <class E, int DP, int DC, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
@@ -435,13 +445,21 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 #pragma unroll
           for (int f = 0; f < DC / 32; ++f)
             o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pb, o[f]);
+          if constexpr (FINE) {
+            const short8 pr = rest<E>(p, pb);
+#pragma unroll
+            for (int f = 0; f < DC / 32; ++f)
+              o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pr, o[f]);
+          }
         }
         // the first probabilities, then a few more beside each product, whose
         // fragments are read two products ahead
-        sched_reads<4>();
-        sched_vector<36>();
-        order<DC / 8 - 2, 2, 6>();
-        sched_mfma<2>();
+        if constexpr (!FINE) {
+          sched_reads<4>();
+          sched_vector<36>();
+          order<DC / 8 - 2, 2, 6>();
+          sched_mfma<2>();
+        }
         __builtin_amdgcn_s_setprio(0);
       }
       __syncthreads();
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 
 // ---- backward: dQ, and D for the other kernel --------------------------
 
-template <class E, int DP, int DC, bool CAUSAL>
+template <class E, int DP, int DC, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
@@ -581,6 +599,13 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
             for (int f = 0; f < DC / 32; ++f)
               dq[f] = E::mfma(at_lane.cols(kt, 32 * kb + 16 * ks, f), b,
                               dq[f]);
+            if constexpr (FINE) {
+              const short8 r = rest<E>(ds + 8 * ks, b);
+#pragma unroll
+              for (int f = 0; f < DC / 32; ++f)
+                dq[f] = E::mfma(at_lane.cols(kt, 32 * kb + 16 * ks, f), r,
+                                dq[f]);
+            }
           }
         }
       }
@@ -619,7 +644,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 
 constexpr int QT = 32;
 
-template <class E, int DP, int DC, bool CAUSAL>
+template <class E, int DP, int DC, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char own_v[OWN * DP * 2];
   __shared__ __attribute__((aligned(16))) char q0[QT * DP * 2];
@@ -731,11 +756,22 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
             dv[f] = E::mfma(at_lane.cols(dt, 16 * ks, f), pb, dv[f]);
             dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sb, dk[f]);
           }
+          if constexpr (FINE) {
+            const short8 pr = rest<E>(p + 8 * ks, pb);
+            const short8 sr = rest<E>(ds + 8 * ks, sb);
+#pragma unroll
+            for (int f = 0; f < DC / 32; ++f) {
+              dv[f] = E::mfma(at_lane.cols(dt, 16 * ks, f), pr, dv[f]);
+              dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sr, dk[f]);
+            }
+          }
         }
-        // reads stay four fragments ahead of the products
-        sched_reads<8>();
-        order<4 * (DC / 32) - 4, 2, 0>();
-        sched_mfma<4>();
+        if constexpr (!FINE) {
+          // reads stay four fragments ahead of the products
+          sched_reads<8>();
+          order<4 * (DC / 32) - 4, 2, 0>();
+          sched_mfma<4>();
+        }
       }
       __syncthreads();
     };
@@ -864,6 +900,15 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   return a;
 }
 
+// A product's second factor, p or dS, is rounded to the type of the first.
+// Over many tokens that costs a fixed 1.4 times what rounding the results
+// costs; over few it swings about that, and where launches bound a call the
+// rest of the rounding can go through a product of its own, which leaves the
+// results' own rounding.  8 heads of 64, forward: 72 tokens 8.4 us (8.6
+// without), 256 tokens 10.6 (9.6), 1024 tokens 23.8 (20.5); with gradients
+// 256 tokens 72 (73), 2048 tokens 132 (119).
+bool is_fine(const Args& a) { return a.T <= 256; }
+
 // Rows stand in LDS as 64 or 128 values; of 128, only 96 are computed with
 // where D is no more (8192 tokens, 16 and 4 heads of 80, causal: 262 us
 // forward and 1032 with gradients, with all 128 288 and 1184).
@@ -873,17 +918,22 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
     auto launch = [&](auto kernel) {                                        \
       hipLaunchKernelGGL(kernel, grid, dim3(NTH), 0, stream.stream(), a);   \
     };                                                                      \
-    auto typed = [&](auto type) {                                           \
+    auto typed = [&](auto type, auto fine) {                                \
       using E = decltype(type);                                             \
-      if (a.D <= 64 && causal) launch(KERNEL<E, 64, 64, true>);             \
-      else if (a.D <= 64) launch(KERNEL<E, 64, 64, false>);                 \
-      else if (a.D <= 96 && causal) launch(KERNEL<E, 128, 96, true>);       \
-      else if (a.D <= 96) launch(KERNEL<E, 128, 96, false>);                \
-      else if (causal) launch(KERNEL<E, 128, 128, true>);                   \
-      else launch(KERNEL<E, 128, 128, false>);                              \
+      constexpr bool F = decltype(fine)::value;                             \
+      if (a.D <= 64 && causal) launch(KERNEL<E, 64, 64, true, F>);          \
+      else if (a.D <= 64) launch(KERNEL<E, 64, 64, false, F>);              \
+      else if (a.D <= 96 && causal) launch(KERNEL<E, 128, 96, true, F>);    \
+      else if (a.D <= 96) launch(KERNEL<E, 128, 96, false, F>);             \
+      else if (causal) launch(KERNEL<E, 128, 128, true, F>);                \
+      else launch(KERNEL<E, 128, 128, false, F>);                           \
     };                                                                      \
-    if (bf) typed(BF());                                                    \
-    else typed(FH());                                                       \
+    auto sized = [&](auto type) {                                           \
+      if (is_fine(a)) typed(type, std::true_type());                        \
+      else typed(type, std::false_type());                                  \
+    };                                                                      \
+    if (bf) sized(BF());                                                    \
+    else sized(FH());                                                       \
   } while (0)
 
 }  // namespace

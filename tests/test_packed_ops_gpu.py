@@ -205,6 +205,55 @@ def test_attention_sharp_scores():
     check_attention([700], 700, 2, 1, 64, FH, scale=1.0, size=1.7, seed=6)
 
 
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("D", [32, 80, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_few_tokens_round_once(causal, D, dtype):
+    """Few tokens: o, dq, dk and dv are off by their own rounding, half a
+    step, and by sums of terms that are off by half a step of half a step
+    (p and dS go in as two values) or by some roundings in 32 bits: 2^-17 of
+    a term's factors.  Terms below the normal fp16 range are off by 2^-24."""
+    half = torch.finfo(dtype).eps / 2
+    fine = max(4 * half * half, 2.0 ** -17)
+    tiny = 2.0 ** -24
+    spans, H, scale = [2, 3, 1, 20, 8, 2, 2, 61, 2, 5], 3, D ** -0.5
+    T = sum(spans)
+    q, k, v, do = (torch.randn(T, h, D, generator=torch.Generator()
+                               .manual_seed(31 + i)).to(dtype)
+                   for i, h in enumerate((H, 1, 1, H)))
+    cu = torch.tensor([0] + spans).cumsum(0)
+    own = [x.cuda().requires_grad_() for x in (q, k, v)]
+    o = flash_attention_packed(*own, cu.to("cuda", torch.int32),
+                               causal=causal)
+    got = [o, *torch.autograd.grad(o, own, do.cuda())]
+    q, k, v, do = (x.double().transpose(0, 1) for x in (q, k, v, do))
+    seq = torch.searchsorted(cu, torch.arange(T), right=True)
+    seen = seq[:, None] == seq
+    if causal:
+        seen = seen.tril()
+    p = ((q @ k.mT) * scale).masked_fill(~seen, -math.inf).softmax(-1)
+    dp = do @ v.mT
+    big = (do.abs() @ v.abs().mT)          # what dP's terms sum to at most
+    Dr = (p * dp).sum(-1, keepdim=True)
+    ds = scale * p * (dp - Dr)
+    most = scale * p * (big + (p * big).sum(-1, keepdim=True))
+    # what each is, and what its terms' factors sum to
+    want = [p @ v, ds @ k, (ds.mT @ q).sum(0, True), (p.mT @ do).sum(0, True)]
+    terms = [p @ v.abs(), most @ k.abs(),
+             (most.mT @ q.abs()).sum(0, True), (p.mT @ do.abs()).sum(0, True)]
+    m = seen.double()
+    lost = [m @ v.abs(), m @ k.abs(), (m @ q.abs()).sum(0, True),
+            (m @ do.abs()).sum(0, True)]
+    if causal:
+        lost[2:] = [(m.mT @ q.abs()).sum(0, True),
+                    (m.mT @ do.abs()).sum(0, True)]
+    for name, g, w, t, n in zip(("o", "dq", "dk", "dv"), got, want, terms,
+                                lost):
+        off = (g.detach().cpu().double().transpose(0, 1) - w).abs()
+        room = half * w.abs() * (1 + half) + fine * t + tiny * (1 + n)
+        assert (off <= room).all(), (name, (off / room).max())
+
+
 def test_attention_late_maximum():
     # the last keys of the first rows are by far the largest
     q, k, v = qkv_of(320, 1, 1, 64, BF, 9)
