@@ -4,9 +4,9 @@
 // rocprim radix-sort + partition/unique kernels.  Those are legal
 // under hipGraph capture, but replaying them from many concurrently
 // captured job graphs proved fragile on ROCm 7 (HSA aperture faults in
-// the captured partition kernel after unrelated allocator traffic —
-// see scripts/repro_prewarm*.py).  These kernels keep the whole
-// embedding path in plain, capture-trivial code:
+// the captured partition kernel after unrelated allocator traffic).
+// These kernels keep the whole embedding path in plain,
+// capture-trivial code:
 //
 // * forward: one vectorized gather pass (short8 = 16 B per lane),
 // * backward: fp32 workspace scatter-add (global atomicAdd — fp32
