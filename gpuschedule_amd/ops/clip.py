@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import Iterable, List, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from ._ext import get_ext
 
@@ -29,6 +30,9 @@ def _cpu_grads(params) -> List[torch.Tensor]:
     grads = [p.grad for p in dict.fromkeys(params) if p.grad is not None]
     if any(g.device.type != "cpu" for g in grads):
         raise RuntimeError("grad_norm: all gradients must be on one device")
+    if any(forward_ad.unpack_dual(g).tangent is not None for g in grads):
+        raise RuntimeError("grad_norm: gradients with a forward-mode "
+                           "tangent are not supported")
     return grads
 
 

@@ -51,7 +51,7 @@ def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
 
     Returns new contiguous ``(q, k)``.  A position outside of the tables
     makes that token's values on that axis NaN.  The tables get no
-    gradient."""
+    gradient, and tangents of theirs are dropped."""
     sections = [int(n) for n in sections]
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] \
             or q.shape[2] != k.shape[2]:

@@ -206,6 +206,9 @@ std::vector<Grad> grads_of(const std::vector<torch::Tensor>& params) {
     TORCH_CHECK(st == torch::kBFloat16 || st == torch::kHalf ||
                     st == torch::kFloat32,
                 "grad_norm: gradients must be bf16, fp16 or fp32, got ", st);
+    TORCH_CHECK(!g._fw_grad(0).defined(),
+                "grad_norm: gradients with a forward-mode tangent are not "
+                "supported");
     if (g.numel() == 0) continue;
     char* at = (char*)g.data_ptr();
     grads.push_back({at, at + g.nbytes(), p.unsafeGetTensorImpl(),

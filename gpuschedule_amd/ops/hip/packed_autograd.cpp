@@ -33,10 +33,15 @@ namespace {
 // Allocations and views inside of a function need no trace of their own.
 using Untraced = at::AutoDispatchBelowADInplaceOrView;
 
+// Whether a call goes through its Function: for a gradient, or because an
+// input carries a forward-mode tangent, which the Function refuses (also
+// without grad mode, which says nothing of tangents).
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool on = at::GradMode::is_enabled();
   for (const auto* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
+    if (t->defined() &&
+        ((on && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined()))
+      return true;
   return false;
 }
 
