@@ -4,8 +4,8 @@
 // sequence i is rows cu[i]..cu[i+1], of which the first lengths[i] are
 // tokens and the rest padding.  Per head, with the keys j that row i sees:
 //   s = scale q.k,  p = exp(s - lse),  lse = log sum exp(s),  o = p v
-//   dV = p^T dO,  dP = dO v^T,  dS = scale p (dP - D),  D = dO.o
-//   dQ = dS k,  dK = dS^T q          (backward computes p again from lse)
+//   dV = p^T dO,  dP = dO v^T,  dS = p (dP - D),  D = dO.o
+//   dQ = scale dS k,  dK = scale dS^T q  (backward computes p again from lse)
 //
 // Matrix work is v_mfma_f32_32x32x16.  Its accumulator holds, in lane l,
 // column l % 32 and rows 8 (i / 4) + 4 (l / 32) + i % 4: a product whose
@@ -37,6 +37,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) unsigned uint4v;
 
 struct BF {
+  static constexpr bool NARROW = false;  // fp32's range
   static __device__ __forceinline__ float16v mfma(short8 a, short8 b,
                                                   float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -56,6 +57,7 @@ struct BF {
 };
 
 struct FH {
+  static constexpr bool NARROW = true;   // 2^-24 to 2^16
   static __device__ __forceinline__ float16v mfma(short8 a, short8 b,
                                                   float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(
@@ -75,6 +77,38 @@ struct FH {
     return (float)__builtin_bit_cast(_Float16, v);
   }
 };
+
+// The other half's value (lane l ^ 32).
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(
+      __builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false,
+      false);
+  // r[0]: the low half's value in both halves, r[1]: the high half's
+  return __builtin_bit_cast(float, threadIdx.x & 32 ? r[0] : r[1]);
+}
+
+// Powers of two for the operands of backward that fp16 could not hold.  p is
+// about 1 / keys and dS = p (dP - D) is as much smaller than dO: unscaled,
+// 2048 tokens with dO of 1e-3 lose 2% of dQ to values under 2^-24.  p <= 1 is
+// held as 2^12 p.  dS goes in as g dS, a g for each accumulator's column:
+// it begins as 2^30 and gives way, the accumulator with it, where a value
+// passes 2^15, so that what is held reaches down to 2^-32 of the largest.
+// The factors, and the scale of the scores, come off the sums in 32 bits.
+constexpr float kPExp = 12.f, kPBy = 0x1p-12f;
+constexpr float kStart = 0x1p30f, kMost = 0x1p15f;
+
+// 1, or what brings the largest of a column's v to between 2^6 and 2^7 if it
+// is over 2^15; both halves of a column get the same.
+template <class E>
+__device__ __forceinline__ float giving_way(const float (&v)[16]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(v[i]));
+  top = fmaxf(top, other_half(top));
+  return top > kMost ? __builtin_amdgcn_ldexpf(
+                           1.f, min(7 - __builtin_amdgcn_frexp_expf(top), 0))
+                     : 1.f;
+}
 
 // What rounding took from 8 values.
 template <class E>
@@ -300,15 +334,6 @@ __device__ __forceinline__ void order() {
   }
 }
 
-// The other half's value (lane l ^ 32).
-__device__ __forceinline__ float other_half(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(
-      __builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false,
-      false);
-  // r[0]: the low half's value in both halves, r[1]: the high half's
-  return __builtin_bit_cast(float, threadIdx.x & 32 ? r[0] : r[1]);
-}
-
 // 2^x; results under 2^-126 are 0
 __device__ __forceinline__ float exp2_of(float x) {
   return __builtin_amdgcn_exp2f(x);
@@ -507,6 +532,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
   float16v dq[DC / 32];
 #pragma unroll
   for (int f = 0; f < DC / 32; ++f) dq[f] = (float16v)(0.f);
+  float g = E::NARROW ? kStart : 1.f, drg = 0.f;  // drg: g D
 
   if (row0 < s.len) {
     short8 q[DC / 16], dO[DC / 16];
@@ -591,7 +617,21 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
           // dS is rounded to the type of k, which the product needs
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            ds[i] = exp2_of(sc[i] * sl2 - lse) * (dp[i] * a.scale - dr);
+            ds[i] = exp2_of(sc[i] * sl2 - lse) *
+                    (E::NARROW ? dp[i] * g - drg : dp[i] - drg);
+          if constexpr (E::NARROW) {
+            const float by = giving_way<E>(ds);
+            if (__any(by < 1.f)) {
+              g *= by;
+              drg *= by;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) ds[i] *= by;
+#pragma unroll
+              for (int f = 0; f < DC / 32; ++f)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dq[f][i] *= by;
+            }
+          }
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             const short8 b = E::pack(ds + 8 * ks);
@@ -621,14 +661,15 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
       dr += other_half(dr);
     }
     if (live && lane < 32) a.drow[(long)head * a.T + at] = -dr;
-    dr *= a.scale;
+    drg = dr * g;
     for (; t < t1; ++t) {
       tile(t, k0, v0, k1, v1);
       if (++t < t1) tile(t, k1, v1, k0, v0);
     }
   }
   if (row < s.rows)
-    put_rows<E, DC>(a.dq + (at * a.H + head) * a.D, live, a.D, lane, 1.f, dq);
+    put_rows<E, DC>(a.dq + (at * a.H + head) * a.D, live, a.D, lane,
+                    a.scale / g, dq);
 }
 
 // ---- backward: dK and dV -----------------------------------------------
@@ -669,6 +710,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
   float16v dk[DC / 32], dv[DC / 32];
 #pragma unroll
   for (int f = 0; f < DC / 32; ++f) dk[f] = dv[f] = (float16v)(0.f);
+  float g = E::NARROW ? kStart * kPBy : 1.f;  // p brings its own factor
 
   if (row0 < s.len) {
     short8 k[DC / 16];
@@ -718,14 +760,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
           (!a.window || r0 <= last + a.window - 1)) {
         float16v sc, dp;           // begin as -lse and -D of their rows
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int r = 8 * g + 4 * (lane >> 5);
+        for (int h = 0; h < 4; ++h) {
+          const int r = 8 * h + 4 * (lane >> 5);
           const float4v ls = *reinterpret_cast<const float4v*>(st + r);
           const float4v dr = *reinterpret_cast<const float4v*>(st + QT + r);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sc[4 * g + j] = ls[j];
-            dp[4 * g + j] = dr[j];
+            sc[4 * h + j] = ls[j];
+            dp[4 * h + j] = dr[j];
           }
         }
 #pragma unroll
@@ -745,8 +787,20 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
         float p[16], ds[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          p[i] = exp2_of(sc[i] * sl2);
-          ds[i] = p[i] * (dp[i] * a.scale);
+          p[i] = exp2_of(E::NARROW ? sc[i] * sl2 + kPExp : sc[i] * sl2);
+          ds[i] = p[i] * (E::NARROW ? dp[i] * g : dp[i]);
+        }
+        if constexpr (E::NARROW) {
+          const float by = giving_way<E>(ds);
+          if (__any(by < 1.f)) {
+            g *= by;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ds[i] *= by;
+#pragma unroll
+            for (int f = 0; f < DC / 32; ++f)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) dk[f][i] *= by;
+          }
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -783,23 +837,27 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
     }
   }
   if (key >= s.rows) return;
+  const float dk_by = E::NARROW ? a.scale * kPBy / g : a.scale;
+  const float dv_by = E::NARROW ? kPBy : 1.f;
   if (a.splits == 1) {
-    put_rows<E, DC>(a.dk + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dk);
-    put_rows<E, DC>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, 1.f, dv);
+    put_rows<E, DC>(a.dk + (at * a.HK + kvh) * a.D, live, a.D, lane, dk_by,
+                    dk);
+    put_rows<E, DC>(a.dv + (at * a.HK + kvh) * a.D, live, a.D, lane, dv_by,
+                    dv);
   } else {
     const long n = (long)a.T * a.HK * a.D;
     float* p = a.part + (2L * split * a.T + at) * a.HK * a.D + kvh * a.D;
 #pragma unroll
     for (int f = 0; f < DC / 32; ++f)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * f + 8 * g + 4 * (lane >> 5);
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * f + 8 * i + 4 * (lane >> 5);
         if (d >= a.D) continue;
         float4v x, y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          x[j] = live ? dk[f][4 * g + j] : 0.f;
-          y[j] = live ? dv[f][4 * g + j] : 0.f;
+          x[j] = live ? dk[f][4 * i + j] * dk_by : 0.f;
+          y[j] = live ? dv[f][4 * i + j] * dv_by : 0.f;
         }
         *reinterpret_cast<float4v*>(p + d) = x;
         *reinterpret_cast<float4v*>(p + n + d) = y;

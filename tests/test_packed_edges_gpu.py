@@ -64,3 +64,87 @@ def test_tangents_are_refused(grad):
         # without tangents the same calls run inside of a dual level
         for call in calls_of(x, w):
             call()
+
+
+# ---- the range of 16 bits --------------------------------------------------
+
+def leaf(t):
+    return t.detach().requires_grad_()
+
+
+def spread(q, k, v, do, causal, scale):
+    """64-bit o, dq, dk, dv of one sequence, and how far each is off as a
+    whole, as the root of a sum of squares: every rounding to the type's
+    relative half step u is off by u / sqrt(3) at most in the mean, and
+    roundings of different values are independent.  What is rounded: p and
+    dS on their way into a product, o (which D = dO.o takes up) and the
+    results; nothing but a result may fall under the type's range."""
+    u = torch.finfo(q.dtype).eps / 2
+    step = torch.finfo(q.dtype).smallest_normal * 2 * u
+    rep = q.shape[1] // k.shape[1]
+    q, k, v, do = (t.detach().double().transpose(0, 1)
+                   for t in (q, k, v, do))
+    kr, vr = (t.repeat_interleave(rep, 0) for t in (k, v))
+    s = (q @ kr.mT) * scale
+    if causal:
+        n = s.shape[-1]
+        s = s.masked_fill(torch.ones(n, n, dtype=torch.bool,
+                                     device=s.device).triu(1), -math.inf)
+    p = s.softmax(-1)
+    o = p @ vr
+    off_o = p.square() @ vr.square() + o.square()
+    off_d = (do.square() * off_o).sum(-1, keepdim=True)
+    ds = p * (do @ vr.mT - (do * o).sum(-1, keepdim=True))
+    dq, dk, dv = scale * (ds @ kr), scale * (ds.mT @ q), p.mT @ do
+    off_q = scale ** 2 * (ds.square() @ kr.square()
+                          + off_d * (p @ kr).square()) + dq.square()
+    off_k = scale ** 2 * (ds.square().mT @ q.square()
+                          + p.square().mT @ (off_d * q.square()))
+    off_v = p.square().mT @ do.square()
+
+    def group(t):
+        return t.unflatten(0, (-1, rep)).sum(1)
+
+    dk, dv = group(dk), group(dv)
+    off_k, off_v = group(off_k) + dk.square(), group(off_v) + dv.square()
+    return [(w.transpose(0, 1),
+             ((u * u * off.sum() + (step / 2) ** 2 * w.numel()) / 3).sqrt())
+            for w, off in ((o, off_o), (dq, off_q), (dk, off_k),
+                           (dv, off_v))]
+
+
+@pytest.mark.parametrize("dtype", [FH, BF])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4])
+def test_attention_small_gradients(size, D, causal, dtype):
+    """Gradients of dO far below 1 keep the precision of their type.  Twice
+    the mean error is allowed: of so many values it hardly strays."""
+    T, H = 2048, 2
+    q, k, v = (leaf(normal((T, n, D), dtype, i))
+               for i, n in enumerate((H, 1, 1)))
+    do = normal((T, H, D), dtype, 3, size)
+    o = flash_attention_packed(q, k, v, cu_of(0, T), causal=causal)
+    got = (o,) + torch.autograd.grad(o, (q, k, v), do)
+    for g, (w, off), name in zip(got, spread(q, k, v, do, causal, D ** -0.5),
+                                 ("o", "dq", "dk", "dv")):
+        err = (g.double() - w).norm()
+        assert err <= 2 * off, f"{name}: {err / off:.3g} of the mean error"
+
+
+def test_attention_large_gradients():
+    """dS over the largest fp16 number, while no result is."""
+    n, T = 3, 300
+    q, k, v, do = (normal((T, 1, 64), FH, i, size) for i, size in
+                   enumerate((1e-3, 1e-3, 100.0, 3000.0)))
+    q, k, v = leaf(q), leaf(k), leaf(v)
+    o = flash_attention_packed(q, k, v, cu_of(*range(0, T + 1, n)))
+    got = (o,) + torch.autograd.grad(o, (q, k, v), do)
+    parts = [spread(*(t[i:i + n] for t in (q, k, v, do)), False, 1 / 8)
+             for i in range(0, T, n)]
+    for g, part, name in zip(got, zip(*parts), ("o", "dq", "dk", "dv")):
+        w = torch.cat([w for w, _ in part])
+        off = torch.stack([e for _, e in part]).norm()
+        assert torch.isfinite(g).all(), name
+        err = (g.double() - w).norm()
+        assert err <= 2 * off, f"{name}: {err / off:.3g} of the mean error"
