@@ -38,6 +38,7 @@ typedef __attribute__((ext_vector_type(4))) unsigned uint4v;
 
 struct BF {
   static constexpr bool NARROW = false;  // fp32's range
+  static constexpr float LIFT = 0.f;     // forward: the largest p is 2^LIFT
   static __device__ __forceinline__ float16v mfma(short8 a, short8 b,
                                                   float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -58,6 +59,7 @@ struct BF {
 
 struct FH {
   static constexpr bool NARROW = true;   // 2^-24 to 2^16
+  static constexpr float LIFT = 7.f;
   static __device__ __forceinline__ float16v mfma(short8 a, short8 b,
                                                   float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(
@@ -439,9 +441,10 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
         top = fmaxf(top, other_half(top)) * sl2;
         // The reference moves only where a maximum leaves it by more than
         // 2^8: o and l are fp32, and probabilities keep their relative
-        // precision up to there, in fp16 too.
-        if (__any(top > m + 8.f)) {
-          const float mn = fmaxf(m, top);
+        // precision up to there.  In fp16 the largest one stands at 2^7 to
+        // 2^15 then: many keys 2^-25 below the largest are still held.
+        if (__any(top > m + (8.f + E::LIFT))) {
+          const float mn = fmaxf(m, top - E::LIFT);
           const float alpha = mn == kNone ? 0.f : exp2_of(m - mn);
           m = mn;
           l *= alpha;

@@ -148,3 +148,31 @@ def test_attention_large_gradients():
         assert torch.isfinite(g).all(), name
         err = (g.double() - w).norm()
         assert err <= 2 * off, f"{name}: {err / off:.3g} of the mean error"
+
+
+@pytest.mark.parametrize("dtype", [FH, BF])
+@pytest.mark.parametrize("T", [200, 2048])
+def test_attention_many_small_probabilities(T, dtype):
+    """One key takes nearly all of each row; what the others hold adds up
+    from probabilities of 2^-25.  Those are off by their own rounding, or by
+    2^-32 of the largest where fp16 has no more; p and o are rounded once
+    each, and 32-bit scores of 17 are off by less than 2^-14 of p."""
+    D = 8
+    q, k, v = (torch.zeros(T, 1, D, device="cuda", dtype=dtype)
+               for _ in range(3))
+    q[..., 0] = 1.0
+    k[7, 0, 0] = 17.25
+    v[:] = normal((T, 1, D), dtype, 1).abs() * 40
+    v[7] = 0
+    o = flash_attention_packed(q, k, v, cu_of(0, T), scale=1.0)
+    p = (q[:, 0].double() @ k[:, 0].double().T).softmax(-1)
+    w = (p @ v[:, 0].double())[:, None]
+    mass = (p @ v[:, 0].double().abs())[:, None]
+    u = torch.finfo(dtype).eps / 2
+    many = v[:, 0].double().abs().sum(0)
+    tiny = 2.0 ** -25 if dtype == FH else 0.0
+    room = u * (mass + w) + 2.0 ** -14 * mass + tiny
+    if dtype == FH:
+        room = room + 2.0 ** -32 * many
+    assert ((o.double() - w).abs() <= room).all()
+    assert (w > 4 * room).all()        # a lost row would show
