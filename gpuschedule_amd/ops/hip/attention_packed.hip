@@ -572,8 +572,12 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     // keys than its two buffers hold, D is the sum of p dP instead (32 rows
     // of 128 tokens, 12 heads of 64: 16.5 us for 13.2; with sequences of 20
     // tokens dQ and dK are off by 1.4 times what rounding their exact values
-    // costs, else by 1.8).
+    // costs, else by 1.8).  So it is in a narrow window, whose tiles are
+    // fetched twice for it (windows of 2, 4, 8 and 16 keys: 1.4 times for
+    // 2.3, 1.8, 1.6 and 1.5; 4096 tokens, 8 and 2 heads of 64, a window of 8:
+    // 50 us for 47, forward and backward).
     const bool few = t1 - t <= 2;
+    const bool narrow = a.window && a.window <= 16;
     auto dots = [&](int t, const char* kt, const char* vt)
         __attribute__((always_inline)) {
       const int kv0 = t * TILE;
@@ -654,15 +658,22 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
       }
       __syncthreads();
     };
+    if (few || narrow) dr = 0.f;
+    if (narrow && !few)
+      for (int i = t; i < t1; ++i) {
+        fetch(i, k0, v0);
+        __syncthreads();
+        dots(i, k0, v0);
+        __syncthreads();
+      }
     fetch(t, k0, v0);
     if (few && t + 1 < t1) fetch(t + 1, k1, v1);
     __syncthreads();
     if (few) {
-      dr = 0.f;
       dots(t, k0, v0);
       if (t + 1 < t1) dots(t + 1, k1, v1);
-      dr += other_half(dr);
     }
+    if (few || narrow) dr += other_half(dr);
     if (live && lane < 32) a.drow[(long)head * a.T + at] = -dr;
     drg = dr * g;
     for (; t < t1; ++t) {
