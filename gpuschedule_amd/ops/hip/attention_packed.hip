@@ -166,6 +166,15 @@ __device__ __forceinline__ bool tile_of(const Args& a, int slot, Seq& s,
   return row0 >= 0 && row0 < s.rows;
 }
 
+// A product's second factor, p or dS, is rounded to the type of the first.
+// Over many tokens that costs a fixed 1.4 times what rounding the results
+// costs; over few it swings about that.  FINE: in a sequence of up to 256
+// tokens the rest of the rounding goes through a product of its own, which
+// leaves the results' own rounding, whatever else the call holds.  Forward
+// and backward, without it: 256 sequences of 32 tokens, 16 and 4 heads of 64,
+// 107 us (96); 40 of 200 tokens, 16 and 4 heads of 128, 196 us (182).
+__device__ __forceinline__ bool is_fine(const Seq& s) { return s.len <= 256; }
+
 // A unit is one slot of one of `heads` kv heads; its `rep` query heads are
 // neighbours in time on one XCD (blocks go to the 8 XCDs in turn), so that
 // they find its keys in that XCD's L2.  Heads change fastest, so that every
@@ -366,11 +375,16 @@ __device__ __forceinline__ bool seen(const Args& a, int key, int row,
 }
 
 // ---- forward -----------------------------------------------------------
-// DP: values of a row in LDS, DC: those that products take.  FINE: second
-// factors go in as two values each, rounded and the rest (`is_fine`).
+// DP: values of a row in LDS, DC: those that products take.
 
-template <class E, int DP, int DC, bool CAUSAL, bool FINE>
-__global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
+// With 128 registers, for four waves on a SIMD, heads of 64 values have their
+// products in a worse order: 8192 tokens, 16 and 4 heads, causal, take 197 us,
+// 175 with three waves (256 sequences of 32 tokens 31 and 36).
+
+template <class E, int DP, int DC, bool CAUSAL>
+__global__ __attribute__((amdgpu_flat_work_group_size(NTH, NTH),
+                          amdgpu_waves_per_eu(2, 3))) void
+packed_fwd_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char k1[TILE * DP * 2];
@@ -409,8 +423,9 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
       stage<DP, TILE>(vp, a.v_t, voff, t * TILE, s.len, a.D, v);
     };
     // One tile, while the next one is on its way to the other buffers.
-    auto tile = [&](int t, const char* kt, const char* vt, char* kn, char* vn)
-        __attribute__((always_inline)) {
+    auto tile = [&](auto fine, int t, const char* kt, const char* vt, char* kn,
+                    char* vn) __attribute__((always_inline)) {
+      constexpr bool FINE = decltype(fine)::value;
       const int kv0 = t * TILE;
       if (t + 1 < t1) fetch(t + 1, kn, vn);
       const int what = sees<CAUSAL>(a, kv0, first, s.len);
@@ -470,14 +485,12 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
           // probabilities are rounded to the type of v, which the matrix
           // product needs; their sum is taken before
           const short8 pb = E::pack(p);
+          [[maybe_unused]] const short8 pr = rest<E>(p, pb);
 #pragma unroll
-          for (int f = 0; f < DC / 32; ++f)
-            o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pb, o[f]);
-          if constexpr (FINE) {
-            const short8 pr = rest<E>(p, pb);
-#pragma unroll
-            for (int f = 0; f < DC / 32; ++f)
-              o[f] = E::mfma(at_lane.cols(vt, 16 * ks, f), pr, o[f]);
+          for (int f = 0; f < DC / 32; ++f) {
+            const short8 vf = at_lane.cols(vt, 16 * ks, f);
+            o[f] = E::mfma(vf, pb, o[f]);
+            if constexpr (FINE) o[f] = E::mfma(vf, pr, o[f]);
           }
         }
         // the first probabilities, then a few more beside each product, whose
@@ -492,13 +505,17 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
       }
       __syncthreads();
     };
-    int t = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
-    fetch(t, k0, v0);
-    __syncthreads();
-    for (; t < t1; ++t) {
-      tile(t, k0, v0, k1, v1);
-      if (++t < t1) tile(t, k1, v1, k0, v0);
-    }
+    auto walk = [&](auto fine) __attribute__((always_inline)) {
+      int t = a.window ? max(row0 - a.window + 1, 0) / TILE : 0;
+      fetch(t, k0, v0);
+      __syncthreads();
+      for (; t < t1; ++t) {
+        tile(fine, t, k0, v0, k1, v1);
+        if (++t < t1) tile(fine, t, k1, v1, k0, v0);
+      }
+    };
+    if (is_fine(s)) walk(std::true_type());
+    else walk(std::false_type());
   }
   l += other_half(l);
   if (row < s.rows) {
@@ -513,7 +530,7 @@ __global__ __launch_bounds__(NTH, 2) void packed_fwd_kernel(const Args a) {
 
 // ---- backward: dQ, and D for the other kernel --------------------------
 
-template <class E, int DP, int DC, bool CAUSAL, bool FINE>
+template <class E, int DP, int DC, bool CAUSAL>
 __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char k0[TILE * DP * 2];
   __shared__ __attribute__((aligned(16))) char v0[TILE * DP * 2];
@@ -598,8 +615,9 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
         }
       }
     };
-    auto tile = [&](int t, const char* kt, const char* vt, char* kn, char* vn)
-        __attribute__((always_inline)) {
+    auto tile = [&](auto fine, int t, const char* kt, const char* vt, char* kn,
+                    char* vn) __attribute__((always_inline)) {
+      constexpr bool FINE = decltype(fine)::value;
       const int kv0 = t * TILE;
       if (!few && t + 1 < t1) fetch(t + 1, kn, vn);
       const int what = sees<CAUSAL>(a, kv0, first, s.len);
@@ -642,16 +660,12 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             const short8 b = E::pack(ds + 8 * ks);
+            [[maybe_unused]] const short8 r = rest<E>(ds + 8 * ks, b);
 #pragma unroll
-            for (int f = 0; f < DC / 32; ++f)
-              dq[f] = E::mfma(at_lane.cols(kt, 32 * kb + 16 * ks, f), b,
-                              dq[f]);
-            if constexpr (FINE) {
-              const short8 r = rest<E>(ds + 8 * ks, b);
-#pragma unroll
-              for (int f = 0; f < DC / 32; ++f)
-                dq[f] = E::mfma(at_lane.cols(kt, 32 * kb + 16 * ks, f), r,
-                                dq[f]);
+            for (int f = 0; f < DC / 32; ++f) {
+              const short8 kf = at_lane.cols(kt, 32 * kb + 16 * ks, f);
+              dq[f] = E::mfma(kf, b, dq[f]);
+              if constexpr (FINE) dq[f] = E::mfma(kf, r, dq[f]);
             }
           }
         }
@@ -676,10 +690,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     if (few || narrow) dr += other_half(dr);
     if (live && lane < 32) a.drow[(long)head * a.T + at] = -dr;
     drg = dr * g;
-    for (; t < t1; ++t) {
-      tile(t, k0, v0, k1, v1);
-      if (++t < t1) tile(t, k1, v1, k0, v0);
-    }
+    auto walk = [&](auto fine) __attribute__((always_inline)) {
+      for (; t < t1; ++t) {
+        tile(fine, t, k0, v0, k1, v1);
+        if (++t < t1) tile(fine, t, k1, v1, k0, v0);
+      }
+    };
+    if (is_fine(s)) walk(std::true_type());
+    else walk(std::false_type());
   }
   if (row < s.rows)
     put_rows<E, DC>(a.dq + (at * a.H + head) * a.D, live, a.D, lane,
@@ -699,8 +717,9 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
 
 constexpr int QT = 32;
 
-template <class E, int DP, int DC, bool CAUSAL, bool FINE>
-__global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
+template <class E, int DP, int DC, bool CAUSAL>
+__global__ __launch_bounds__(NTH, DP == 64 ? 3 : 2) void packed_bwd_kv_kernel(
+    const Args a) {
   __shared__ __attribute__((aligned(16))) char own_v[OWN * DP * 2];
   __shared__ __attribute__((aligned(16))) char q0[QT * DP * 2];
   __shared__ __attribute__((aligned(16))) char d0[QT * DP * 2];
@@ -761,8 +780,10 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
     long n = all * split / a.splits;
     const long stop = all * (split + 1) / a.splits;
     int head = kvh * rep + (int)(n / tiles), t = t1 - 1 - (int)(n % tiles);
-    auto tile = [&](const char* qt, const char* dt, const float* st, char* qn,
-                    char* dn, float* sn) __attribute__((always_inline)) {
+    auto tile = [&](auto fine, const char* qt, const char* dt, const float* st,
+                    char* qn, char* dn, float* sn)
+        __attribute__((always_inline)) {
+      constexpr bool FINE = decltype(fine)::value;
       const int r0 = t * QT;
       at_lane.again();
       if (--t < t0) {
@@ -819,18 +840,17 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
           const short8 pb = E::pack(p + 8 * ks), sb = E::pack(ds + 8 * ks);
+          [[maybe_unused]] const short8 pr = rest<E>(p + 8 * ks, pb);
+          [[maybe_unused]] const short8 sr = rest<E>(ds + 8 * ks, sb);
 #pragma unroll
           for (int f = 0; f < DC / 32; ++f) {
-            dv[f] = E::mfma(at_lane.cols(dt, 16 * ks, f), pb, dv[f]);
-            dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sb, dk[f]);
-          }
-          if constexpr (FINE) {
-            const short8 pr = rest<E>(p + 8 * ks, pb);
-            const short8 sr = rest<E>(ds + 8 * ks, sb);
-#pragma unroll
-            for (int f = 0; f < DC / 32; ++f) {
-              dv[f] = E::mfma(at_lane.cols(dt, 16 * ks, f), pr, dv[f]);
-              dk[f] = E::mfma(at_lane.cols(qt, 16 * ks, f), sr, dk[f]);
+            const short8 df = at_lane.cols(dt, 16 * ks, f);
+            const short8 qf = at_lane.cols(qt, 16 * ks, f);
+            dv[f] = E::mfma(df, pb, dv[f]);
+            dk[f] = E::mfma(qf, sb, dk[f]);
+            if constexpr (FINE) {
+              dv[f] = E::mfma(df, pr, dv[f]);
+              dk[f] = E::mfma(qf, sr, dk[f]);
             }
           }
         }
@@ -845,10 +865,14 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_kv_kernel(const Args a) {
     };
     if (n < stop) fetch(head, t, q0, d0, s0);
     __syncthreads();
-    while (n < stop) {
-      tile(q0, d0, s0, q1, d1, s1);
-      if (n < stop) tile(q1, d1, s1, q0, d0, s0);
-    }
+    auto walk = [&](auto fine) __attribute__((always_inline)) {
+      while (n < stop) {
+        tile(fine, q0, d0, s0, q1, d1, s1);
+        if (n < stop) tile(fine, q1, d1, s1, q0, d0, s0);
+      }
+    };
+    if (is_fine(s)) walk(std::true_type());
+    else walk(std::false_type());
   }
   if (key >= s.rows) return;
   const float dk_by = E::NARROW ? a.scale * kPBy / g : a.scale;
@@ -972,15 +996,6 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   return a;
 }
 
-// A product's second factor, p or dS, is rounded to the type of the first.
-// Over many tokens that costs a fixed 1.4 times what rounding the results
-// costs; over few it swings about that, and where launches bound a call the
-// rest of the rounding can go through a product of its own, which leaves the
-// results' own rounding.  8 heads of 64, forward: 72 tokens 8.4 us (8.6
-// without), 256 tokens 10.6 (9.6), 1024 tokens 23.8 (20.5); with gradients
-// 256 tokens 72 (73), 2048 tokens 132 (119).
-bool is_fine(const Args& a) { return a.T <= 256; }
-
 // Rows stand in LDS as 64 or 128 values; of 128, only 96 are computed with
 // where D is no more (8192 tokens, 16 and 4 heads of 80, causal: 262 us
 // forward and 1032 with gradients, with all 128 288 and 1184).
@@ -990,22 +1005,17 @@ bool is_fine(const Args& a) { return a.T <= 256; }
     auto launch = [&](auto kernel) {                                        \
       hipLaunchKernelGGL(kernel, grid, dim3(NTH), 0, stream.stream(), a);   \
     };                                                                      \
-    auto typed = [&](auto type, auto fine) {                                \
+    auto typed = [&](auto type) {                                           \
       using E = decltype(type);                                             \
-      constexpr bool F = decltype(fine)::value;                             \
-      if (a.D <= 64 && causal) launch(KERNEL<E, 64, 64, true, F>);          \
-      else if (a.D <= 64) launch(KERNEL<E, 64, 64, false, F>);              \
-      else if (a.D <= 96 && causal) launch(KERNEL<E, 128, 96, true, F>);    \
-      else if (a.D <= 96) launch(KERNEL<E, 128, 96, false, F>);             \
-      else if (causal) launch(KERNEL<E, 128, 128, true, F>);                \
-      else launch(KERNEL<E, 128, 128, false, F>);                           \
+      if (a.D <= 64 && causal) launch(KERNEL<E, 64, 64, true>);             \
+      else if (a.D <= 64) launch(KERNEL<E, 64, 64, false>);                 \
+      else if (a.D <= 96 && causal) launch(KERNEL<E, 128, 96, true>);       \
+      else if (a.D <= 96) launch(KERNEL<E, 128, 96, false>);                \
+      else if (causal) launch(KERNEL<E, 128, 128, true>);                   \
+      else launch(KERNEL<E, 128, 128, false>);                              \
     };                                                                      \
-    auto sized = [&](auto type) {                                           \
-      if (is_fine(a)) typed(type, std::true_type());                        \
-      else typed(type, std::false_type());                                  \
-    };                                                                      \
-    if (bf) sized(BF());                                                    \
-    else sized(FH());                                                       \
+    if (bf) typed(BF());                                                    \
+    else typed(FH());                                                       \
   } while (0)
 
 }  // namespace

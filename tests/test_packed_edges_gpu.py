@@ -199,3 +199,31 @@ def test_attention_narrow_window(window, D, dtype):
                                  ("o", "dq", "dk", "dv")):
         err = (g.double() - w).norm()
         assert err <= off, f"{name}: {err / off:.3g} of the mean error"
+
+
+# ---- a sequence by itself and among others ---------------------------------
+
+@pytest.mark.parametrize("dtype", [FH, BF])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_does_not_depend_on_the_batch(causal, D, dtype):
+    """A sequence has the same bits alone and behind others (of gradients of
+    k and v where both calls sum without splits, as over short sequences)."""
+    for spans, whole in (([40] * 25, True), ([300, 40, 700, 256, 5], False),
+                         ([3000, 17, 100], False)):
+        T = sum(spans)
+        q, k, v, do = (normal((T, n, D), dtype, i)
+                       for i, n in enumerate((4, 2, 2, 4)))
+        q, k, v = leaf(q), leaf(k), leaf(v)
+        cu = [sum(spans[:i]) for i in range(len(spans) + 1)]
+        o = flash_attention_packed(q, k, v, cu_of(*cu), causal=causal)
+        got = (o,) + torch.autograd.grad(o, (q, k, v), do)
+        for b, e in zip(cu[:-1], cu[1:]):
+            if e - b > 256:
+                continue
+            part = [leaf(t[b:e]) for t in (q, k, v)]
+            o = flash_attention_packed(*part, cu_of(0, e - b), causal=causal)
+            alone = (o,) + torch.autograd.grad(o, part, do[b:e])
+            for x, y, name in zip(got, alone, ("o", "dq", "dk", "dv")):
+                if whole or name in ("o", "dq"):
+                    assert torch.equal(x[b:e], y), (name, e - b)
