@@ -152,8 +152,8 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor,
     fp16, D a multiple of 8 up to 128; slices of a fused projection are
     read in place.  ``cu_seqlens`` int32 [sequences + 1], on q's device:
     sequence i is rows ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``; it
-    begins with 0 and does not fall, and rows behind its last value
-    belong to no sequence.  ``lengths`` int32 [sequences]: only the
+    does not fall, and rows in front of its first value (0, if all are
+    used) or behind its last belong to no sequence.  ``lengths`` int32 [sequences]: only the
     first ``lengths[i]`` rows of sequence i are tokens, the rest is
     padding (a padded batch [B, S] is ``cu_seqlens = [0, S, 2S, ...]``).
 

@@ -18,12 +18,12 @@
 // probabilities never pass through LDS, and no transposed copy is made.
 //
 // Sequences are found on the GPU: a call waits for nothing and can be
-// captured.  A tile of R rows lies in one sequence; sequence i owns the
-// slots from cu[i] / R + i on, which is at least as many as it has tiles,
-// so that a slot's sequence is a binary search over cu and the number of
-// slots, T / R + sequences + 1, is known on the host.  Rows behind the last
-// sequence count as one more, without tokens.  Rows without tokens get
-// zeros.
+// captured.  A tile of R rows lies in one sequence; sequence i of those that
+// begin at b[i] owns the slots from b[i] / R + i on, which is at least as many
+// as it has tiles, so that a slot's sequence is a binary search over b and the
+// number of slots, T / R + sequences + 2, is known on the host.  Rows in front
+// of the first sequence and rows behind the last count as one more each,
+// without tokens.  Rows without tokens get zeros.
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -145,23 +145,25 @@ struct Seq {
   int begin, rows, len;            // first row, all rows, tokens
 };
 
+// Where sequence i begins: 1 to B are the caller's, 0 and B + 1 the rows in
+// front of them and behind them.
 __device__ __forceinline__ int bound_of(const Args& a, int i) {
-  return i > a.B ? a.T : min(max(a.cu[i], 0), a.T);
+  return i == 0 ? 0 : i > a.B + 1 ? a.T : min(max(a.cu[i - 1], 0), a.T);
 }
 
 // The sequence and first row (in it) of a slot; false: the slot is not used.
 template <int R>
 __device__ __forceinline__ bool tile_of(const Args& a, int slot, Seq& s,
                                         int& row0) {
-  int lo = 0, hi = a.B;            // the last i whose slots begin at or before
+  int lo = 0, hi = a.B + 1;        // the last i whose slots begin at or before
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
     if (bound_of(a, mid) / R + mid <= slot) lo = mid; else hi = mid - 1;
   }
   s.begin = bound_of(a, lo);
   s.rows = max(bound_of(a, lo + 1) - s.begin, 0);
-  s.len = lo == a.B ? 0 : s.rows;
-  if (a.lengths && lo < a.B) s.len = min(max(a.lengths[lo], 0), s.rows);
+  s.len = lo == 0 || lo > a.B ? 0 : s.rows;
+  if (a.lengths && s.len) s.len = min(max(a.lengths[lo - 1], 0), s.rows);
   row0 = (slot - (s.begin / R + lo)) * R;
   return row0 >= 0 && row0 < s.rows;
 }
@@ -988,7 +990,7 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   a.D = (int)q.size(2);
   a.window = (int)std::min<int64_t>(window, a.T);
   a.scale = (float)scale;
-  const long slots = (long)a.T / OWN + a.B + 1;
+  const long slots = (long)a.T / OWN + a.B + 2;
   TORCH_CHECK(slots * a.H < (1L << 30),
               "attn_packed: too many rows and heads");
   a.slots = (int)slots;

@@ -227,3 +227,33 @@ def test_attention_does_not_depend_on_the_batch(causal, D, dtype):
             for x, y, name in zip(got, alone, ("o", "dq", "dk", "dv")):
                 if whole or name in ("o", "dq"):
                     assert torch.equal(x[b:e], y), (name, e - b)
+
+
+# ---- rows of no sequence ---------------------------------------------------
+
+@pytest.mark.parametrize("T,cu", [(300, (5, 105, 300)), (700, (300, 301)),
+                                  (520, (128, 128, 390, 400)), (64, (64, 64)),
+                                  (200, (130, 200))])
+@pytest.mark.parametrize("padded", [False, True])
+def test_attention_rows_in_front(padded, T, cu):
+    """cu_seqlens may begin behind the first row: rows in front of it get
+    zeros, the others what they get without those rows."""
+    q, k, v, do = (normal((T, n, 64), BF, i)
+                   for i, n in enumerate((4, 2, 2, 4)))
+    lengths = torch.tensor([max(b - a - 3, 0) for a, b in zip(cu, cu[1:])],
+                           dtype=torch.int32, device="cuda") \
+        if padded else None
+    for t in (q, k, v, do):
+        t[:cu[0]] = math.nan
+    q, k, v = leaf(q), leaf(k), leaf(v)
+    # memory that is handed out next holds no zeros
+    junk = torch.full((T * 64 * 4 * 8,), math.nan, device="cuda", dtype=BF)
+    del junk
+    o = flash_attention_packed(q, k, v, cu_of(*cu), lengths, causal=True)
+    got = (o,) + torch.autograd.grad(o, (q, k, v), do)
+    part = [leaf(t[cu[0]:]) for t in (q, k, v)]
+    o = flash_attention_packed(*part, cu_of(*(n - cu[0] for n in cu)),
+                               lengths, causal=True)
+    rest = (o,) + torch.autograd.grad(o, part, do[cu[0]:])
+    for x, y in zip(got, rest):
+        assert (x[:cu[0]] == 0).all() and torch.equal(x[cu[0]:], y)
