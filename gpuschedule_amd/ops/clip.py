@@ -25,6 +25,11 @@ def _with_grad(parameters):
     return params, None
 
 
+def _nothing(params) -> torch.Tensor:
+    return torch.zeros((), dtype=torch.float32,
+                       device=params[0].device if params else "cpu")
+
+
 def _cpu_grads(params) -> List[torch.Tensor]:
     # a tied weight counts once
     grads = [p.grad for p in dict.fromkeys(params) if p.grad is not None]
@@ -43,7 +48,8 @@ def _cpu_norm(grads) -> torch.Tensor:
 def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]
               ) -> torch.Tensor:
     """The 2-norm of all gradients of ``parameters`` taken together, as
-    an fp32 scalar tensor on their device (0 if there are none).
+    an fp32 scalar tensor on their device (0, on the parameters' device,
+    if there are none).
 
     Gradients may mix bf16, fp16 and fp32.  They must be on one device,
     dense in memory (any order of dimensions), and must not share
@@ -51,7 +57,7 @@ def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]
     summed in 64 bits."""
     params, any_grad = _with_grad(parameters)
     if any_grad is None:
-        return torch.zeros(())
+        return _nothing(params)
     if any_grad.is_cuda:
         return get_ext(required=True).grad_norm_clip(params, -1.0)
     return _cpu_norm(_cpu_grads(params)).float()
@@ -73,7 +79,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]],
                          f"got {max_norm}")
     params, any_grad = _with_grad(parameters)
     if any_grad is None:
-        return torch.zeros(())
+        return _nothing(params)
     if any_grad.is_cuda:
         return get_ext(required=True).grad_norm_clip(params, max_norm)
     grads = _cpu_grads(params)

@@ -63,3 +63,18 @@ def test_attention_slots_cover_all_rows(T, B):
         wild = torch.randint(-T - 9, 2 * T + 9, (B + 1,), generator=gen)
         for b, e in tiles(wild.tolist()):
             assert 0 <= b <= e <= T
+
+
+def test_no_gradients_at_all():
+    """0 as any other norm comes: fp32, on the parameters' device."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float64)
+    try:
+        for device in ("cpu", "meta"):
+            p = torch.nn.Parameter(torch.empty(3, device=device))
+            for n in (grad_norm([p]), clip_grad_norm_(iter([p, p]), 1.0)):
+                assert n.dtype == torch.float32 and n.device.type == device
+                assert n.shape == ()
+        assert grad_norm([]).dtype == torch.float32 and grad_norm([]) == 0
+    finally:
+        torch.set_default_dtype(before)
