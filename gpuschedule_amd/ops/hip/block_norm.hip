@@ -279,16 +279,29 @@ __device__ __forceinline__ void block_add(float (&v)[E], float* room) {
   }
 }
 
+// Waves on a SIMD that the backward kernel leaves registers for (512 / waves).
+// 16-bit rows fit 128 but for a few; of an odd width and with whole groups
+// they need three waves' (12474 rows of 1001 bf16, a gate for each, forward
+// and backward: 117 us, 134 with four waves, where 35 registers spill), and
+// so do 32-bit rows (1024 fp32: 144 us for 169).  Blocks of 512 threads have
+// 128 registers or 256: 32-bit rows take 256 (4096 rows of 4096 fp32, a gate
+// for each: 173 us, 227 with 128, where up to 47 spill), 16-bit ones do as
+// well with 128 (4000 rows of 4001: 175 us), though 37 spill at an odd width
+// with whole groups.  Blocks of 1024 threads have no more than 128: 13 to 68
+// spill with 8 values a thread, and 136 to 504 with 16.
+template <class T, int ROWT, bool EVEN, bool WHOLE>
+constexpr int BWD_WAVES =
+    sizeof(T) == 4 ? (ROWT > 512 ? 4 : ROWT > 256 ? 2 : 3)
+                   : (ROWT <= 256 && !EVEN && WHOLE ? 3 : 4);
+
 // A block's workers (a worker: the ROWT threads of a row) leave one partial
 // row of each sum.  WHOLE: a worker takes `per` rows that are whole groups,
 // and finishes their rows of dg.  Otherwise `slices` blocks share a group of
 // rows, `per` rows each, which the workers take in turn, and sum(e hh) of
 // the group is left in parts too.
-// 16-bit rows fit four waves on a SIMD (128 registers); 32-bit ones spill
-// there, and are faster with three: 12474 rows of 1024, a gate for each, 169
-// us forward and backward with four, 144 with three.
 template <class T, int ROWT, int E, bool EVEN, bool WHOLE>
-__global__ __launch_bounds__(BLOCK<ROWT>, sizeof(T) == 2 || ROWT > 256 ? 4 : 3)
+__global__
+__launch_bounds__(BLOCK<ROWT>, (BWD_WAVES<T, ROWT, EVEN, WHOLE>))
 void block_norm_bwd_kernel(
     const T* __restrict__ dn, const T* __restrict__ ds,
     const T* __restrict__ h, const T* __restrict__ x,
