@@ -257,3 +257,89 @@ def test_attention_rows_in_front(padded, T, cu):
     rest = (o,) + torch.autograd.grad(o, part, do[cu[0]:])
     for x, y in zip(got, rest):
         assert (x[:cu[0]] == 0).all() and torch.equal(x[cu[0]:], y)
+
+
+# ---- together --------------------------------------------------------------
+
+class Rounded(torch.autograd.Function):
+    """To bf16 and back, and its gradient too, as between two operators."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.to(BF).to(x.dtype)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g.to(BF).to(g.dtype)
+
+
+def plain_block(x, params, cu, angle, r):
+    """One block of packed tokens in 64 bits, `r` behind every operator."""
+    wqkv, wo, w1, w2, g = params
+    T, D = x.shape[0], 64
+    q, k, v = r(x @ wqkv).split([256, 128, 128], -1)
+    q, k, v = (t.unflatten(-1, (-1, D)).transpose(0, 1) for t in (q, k, v))
+    q, k = (r(torch.cat([t[..., :32] * angle.cos() - t[..., 32:] * angle.sin(),
+                         t[..., 32:] * angle.cos() + t[..., :32] * angle.sin()],
+                        -1)) for t in (q, k))
+    k, v = (t.repeat_interleave(2, 0) for t in (k, v))
+    row = torch.arange(T, device=x.device)
+    seq = torch.searchsorted(cu.long(), row, right=True)
+    seen = (seq[:, None] == seq) & (seq <= len(cu) - 1) & (row <= row[:, None])
+    s = (q @ k.mT / 8).masked_fill(~seen, -1e300)
+    o = r((s.softmax(-1) * seen) @ v).transpose(0, 1).reshape(T, 256)
+    h = r(o @ wo)
+    S = 0.9 * x + g * h * (h.square().mean(-1, keepdim=True)
+                           + 1e-6).rsqrt() * w1
+    return S * (S.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w2, S
+
+
+def test_together_each_gradient_by_itself():
+    """rope, attention, block norm and clipping in one step: every
+    parameter's gradient, and the q, k and v columns by themselves, against
+    64 bits.  What they may be off is what bf16 between the operators costs,
+    taken from the same 64-bit step with that rounding; its errors are other
+    ones of the same size, and twice their norm is allowed."""
+    T = 300
+    x = normal((T, 256), BF, 0)
+    params = [normal((256, 512), BF, 1, 0.06), normal((256, 256), BF, 2, 0.06)]
+    params += [(1 + normal((256,), FP, 3 + i, 0.2)).to(BF) for i in range(3)]
+    params = [torch.nn.Parameter(p) for p in params]
+    cu, pos = cu_of(0, 120, 120, 270), torch.randint(
+        0, 400, (3, T), generator=torch.Generator().manual_seed(5)).cuda()
+    inv = 1e4 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    table = torch.outer(torch.arange(400, dtype=torch.float64), inv).cuda()
+    out_grads = normal((T, 256), BF, 7), normal((T, 256), BF, 8)
+
+    wqkv, wo, w1, w2, g = params
+    q, k, v = (x @ wqkv).split([256, 128, 128], -1)
+    q, k, v = (t.unflatten(-1, (-1, 64)) for t in (q, k, v))
+    q, k = fused_rope_axes(q, k, pos, table.cos().float(),
+                           table.sin().float(), [8, 12, 12])
+    o = flash_attention_packed(q, k, v, cu, causal=True)
+    out = fused_block_norm(o.reshape(T, 256) @ wo, x, w1, w2, g, 0.9)
+    for p, grad in zip(params, torch.autograd.grad(out, params, out_grads)):
+        p.grad = grad
+    total = clip_grad_norm_(params, 1.0)
+
+    axis = torch.tensor([0] * 8 + [1] * 12 + [2] * 12, device="cuda")
+    angle = table[pos[axis].t(), torch.arange(32, device="cuda")]
+    grads = []
+    for r in (lambda t: t, Rounded.apply):
+        p64 = [p.detach().double().requires_grad_() for p in params]
+        res = plain_block(x.double(), p64, cu, angle, r)
+        grads.append(torch.autograd.grad(
+            res, p64, [t.double() for t in out_grads]))
+    want = sum(t.square().sum() for t in grads[0]) ** 0.5
+    assert (total.double() - want).abs() <= 2 ** -6 * want
+    names = ["q", "k", "v", "wo", "post", "pre", "gate"]
+
+    def parts(ts):
+        return [*ts[0].split([256, 128, 128], -1), *ts[1:]]
+
+    for name, got, exact, rounded in zip(names, parts(
+            [p.grad.double() for p in params]), *map(parts, grads)):
+        off = (Rounded.apply(rounded) - exact).norm()
+        assert 0 < off <= 0.05 * exact.norm(), name   # it says something
+        err = (got * total.double() - exact).norm()
+        assert err <= 2 * off, f"{name}: {err / off:.3g} of bf16's error"
