@@ -165,7 +165,8 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor,
     in o and in the gradients, whatever they hold.  An infinity or NaN
     stays in its own sequence.  Where cu_seqlens falls or leaves [0, T]
     the result is undefined, but nothing outside the tensors is
-    touched.  Nothing here waits for the GPU; a call can be captured."""
+    touched.  Nothing here waits for the GPU; a call can be captured.
+    (T / 128 + sequences) * H has to stay under 2^24."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape \
             or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError(f"flash_attention_packed: q [T, H, D], k and v "

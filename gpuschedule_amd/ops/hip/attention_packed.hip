@@ -991,8 +991,10 @@ Args args_of(const torch::Tensor& q, const torch::Tensor& k,
   a.window = (int)std::min<int64_t>(window, a.T);
   a.scale = (float)scale;
   const long slots = (long)a.T / OWN + a.B + 2;
-  TORCH_CHECK(slots * a.H < (1L << 30),
-              "attn_packed: too many rows and heads");
+  // a launch has less than 2^32 threads; heads are rounded up to 8 units
+  TORCH_CHECK((slots + 8) * a.H * NTH < (1L << 32),
+              "attn_packed: too many rows, sequences and heads: (rows / 128 + "
+              "sequences + 10) * heads must be less than 2^24");
   a.slots = (int)slots;
   a.splits = 1;
   return a;

@@ -343,3 +343,16 @@ def test_together_each_gradient_by_itself():
         assert 0 < off <= 0.05 * exact.norm(), name   # it says something
         err = (got * total.double() - exact).norm()
         assert err <= 2 * off, f"{name}: {err / off:.3g} of bf16's error"
+
+
+def test_attention_too_many_blocks_are_refused():
+    """More threads than a launch may have, before anything is allocated."""
+    q = torch.zeros(1, 32, 8, device="cuda", dtype=BF).expand(1 << 27, 32, 8)
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(RuntimeError, match="too many rows"):
+        flash_attention_packed(q, q, q, cu_of(0, 1 << 27))
+    many = torch.zeros(1 << 23, device="cuda", dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        flash_attention_packed(q[:1], q[:1], q[:1], many)
+    del many
+    assert torch.cuda.memory_allocated() <= before + 4096
