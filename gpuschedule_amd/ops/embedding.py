@@ -5,7 +5,8 @@ one-pass vectorized gather, the point is the BACKWARD: torch's dense
 embedding backward runs rocprim radix-sort/partition kernels whose
 hipGraph replay proved fragile on ROCm 7 when many job graphs coexist
 (HSA aperture faults).  The HIP path is two plain kernels (fp32 atomic
-scatter + cast) that capture and replay trivially.  CPU path: fp32 torch reference (tests)."""
+scatter + cast) that capture and replay trivially.  CPU path: fp32
+torch reference (tests)."""
 from __future__ import annotations
 
 import torch

@@ -89,7 +89,8 @@ __device__ __forceinline__ float other_half(float v) {
   return __builtin_bit_cast(float, threadIdx.x & 32 ? r[0] : r[1]);
 }
 
-// Powers of two for the operands of backward that fp16 could not hold.  p is
+// Powers of two for the operands of backward that fp16 could not hold (8192
+// tokens, 16 and 4 heads of 128, training: 3-4% of the time).  p is
 // about 1 / keys and dS = p (dP - D) is as much smaller than dO: unscaled,
 // 2048 tokens with dO of 1e-3 lose 2% of dQ to values under 2^-24.  p <= 1 is
 // held as 2^12 p.  dS goes in as g dS, a g for each accumulator's column:
@@ -588,13 +589,13 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     // D = dO.o carries the rounding of o, and of the probabilities that went
     // into it: next to nothing where many keys share a row, but with few it
     // is half of the error of dQ and dK.  Where a block's rows see no more
-    // keys than its two buffers hold, D is the sum of p dP instead (32 rows
-    // of 128 tokens, 12 heads of 64: 16.5 us for 13.2; with sequences of 20
-    // tokens dQ and dK are off by 1.4 times what rounding their exact values
-    // costs, else by 1.8).  So it is in a narrow window, whose tiles are
-    // fetched twice for it (windows of 2, 4, 8 and 16 keys: 1.4 times for
-    // 2.3, 1.8, 1.6 and 1.5; 4096 tokens, 8 and 2 heads of 64, a window of 8:
-    // 50 us for 47, forward and backward).
+    // keys than its two buffers hold, D is the sum of p dP instead (3 us more
+    // for 32 rows of 128 tokens, 12 heads of 64; with sequences of 20 tokens
+    // dQ and dK are off by what rounding their exact values costs, else by
+    // 1.1 times that).  So it is in a narrow window, whose tiles are fetched
+    // twice for it (windows of 2, 4, 8 and 16 keys in longer sequences: 1.4
+    // times for 2.3, 1.8, 1.6 and 1.5; 4096 tokens, 8 and 2 heads of 64, a
+    // window of 8: 50 us for 47, forward and backward).
     const bool few = t1 - t <= 2;
     const bool narrow = a.window && a.window <= 16;
     auto dots = [&](int t, const char* kt, const char* vt)

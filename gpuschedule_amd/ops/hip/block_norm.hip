@@ -285,9 +285,10 @@ __device__ __forceinline__ void block_add(float (&v)[E], float* room) {
 // and backward: 117 us, 134 with four waves, where 35 registers spill), and
 // so do 32-bit rows (1024 fp32: 144 us for 169).  Blocks of 512 threads have
 // 128 registers or 256: 32-bit rows take 256 (4096 rows of 4096 fp32, a gate
-// for each: 173 us, 227 with 128, where up to 47 spill), 16-bit ones do as
-// well with 128 (4000 rows of 4001: 175 us), though 37 spill at an odd width
-// with whole groups.  Blocks of 1024 threads have no more than 128: 13 to 68
+// for each: 173 us, 227 with 128, where up to 47 spill), 16-bit ones keep
+// 128, though 37 spill at an odd width with whole groups: with 256, 4000 rows
+// of 4001 and a gate for each take 151 us for 175, but 700 groups of 10 rows
+// 307 for 278.  Blocks of 1024 threads have no more than 128: 13 to 68
 // spill with 8 values a thread, and 136 to 504 with 16.
 template <class T, int ROWT, bool EVEN, bool WHOLE>
 constexpr int BWD_WAVES =
