@@ -4,6 +4,7 @@ from __future__ import annotations
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from ._ext import get_ext
 
@@ -51,7 +52,7 @@ def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
 
     Returns new contiguous ``(q, k)``.  A position outside of the tables
     makes that token's values on that axis NaN.  The tables get no
-    gradient, and tangents of theirs are dropped."""
+    gradient, and may carry no forward-mode tangent."""
     sections = [int(n) for n in sections]
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] \
             or q.shape[2] != k.shape[2]:
@@ -83,6 +84,10 @@ def fused_rope_axes(q: torch.Tensor, k: torch.Tensor,
     if q.is_cuda:
         return tuple(get_ext(required=True).rope_axes(
             q, k, positions, cosb, sinb, sections))
+    if any(forward_ad.unpack_dual(t).tangent is not None
+           for t in (cosb, sinb)):
+        raise RuntimeError("fused_rope_axes: tables with a forward-mode "
+                           "tangent are not supported")
     cosb, sinb = cosb.detach(), sinb.detach()
     axis = torch.repeat_interleave(torch.arange(len(sections)),
                                    torch.tensor(sections))

@@ -182,6 +182,9 @@ std::vector<Tensor> rope_axes_grad(Tensor q, Tensor k, Tensor pos,
   q = dense_rows(q);
   k = dense_rows(k);
   pos = pos.contiguous();
+  TORCH_CHECK(!cosb._fw_grad(0).defined() && !sinb._fw_grad(0).defined(),
+              "fused_rope_axes: tables with a forward-mode tangent are not "
+              "supported");
   cosb = cosb.detach().contiguous();
   sinb = sinb.detach().contiguous();
   if (!wants_grad({&q, &k}))

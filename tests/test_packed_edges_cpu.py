@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 from gpuschedule_amd.ops import (clip_grad_norm_, flash_attention_packed,
-                                 grad_norm)
+                                 fused_rope_axes, grad_norm)
 
 
 def test_clip_refuses_tangents():
@@ -15,6 +15,18 @@ def test_clip_refuses_tangents():
             with pytest.raises(RuntimeError, match="tangent"):
                 call([p])
         assert (p.grad == 1).all()
+
+
+def test_rope_refuses_tangents_of_tables():
+    q, pos = torch.randn(3, 1, 8), torch.zeros(1, 3, dtype=torch.int64)
+    c = torch.ones(2, 4)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(c, torch.ones(2, 4))
+        for tables in ((d, c), (c, d)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                fused_rope_axes(q, q, pos, *tables, [4])
+        y, _ = fused_rope_axes(forward_ad.make_dual(q, q), q, pos, c, c, [4])
+        assert forward_ad.unpack_dual(y).tangent is not None
 
 
 def test_attention_rows_in_front():

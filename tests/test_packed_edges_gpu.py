@@ -61,6 +61,12 @@ def test_tangents_are_refused(grad):
         for call in (grad_norm, lambda q: clip_grad_norm_(q, 0.1)):
             with pytest.raises(RuntimeError, match="tangent"):
                 call([p])
+        cos = torch.ones(2, 4, device="cuda")
+        pos = torch.zeros(1, 6, dtype=torch.int64, device="cuda")
+        table = forward_ad.make_dual(cos, torch.ones_like(cos))
+        for tables in ((table, cos), (cos, table)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                fused_rope_axes(x, x, pos, *tables, [4])
         # without tangents the same calls run inside of a dual level
         for call in calls_of(x, w):
             call()
