@@ -593,11 +593,12 @@ __global__ __launch_bounds__(NTH, 2) void packed_bwd_q_kernel(const Args a) {
     // for 32 rows of 128 tokens, 12 heads of 64; with sequences of 20 tokens
     // dQ and dK are off by what rounding their exact values costs, else by
     // 1.1 times that).  So it is in a narrow window, whose tiles are fetched
-    // twice for it (windows of 2, 4, 8 and 16 keys in longer sequences: 1.4
-    // times for 2.3, 1.8, 1.6 and 1.5; 4096 tokens, 8 and 2 heads of 64, a
-    // window of 8: 50 us for 47, forward and backward).
+    // twice for it (windows of 2, 4, 8 and 32 keys in longer sequences: 1.4
+    // times for 2.3, 1.8, 1.6 and 1.5; 4096 tokens, 8 and 2 heads of 64,
+    // forward and backward: 51 us for 47 with a window of 8, 50 for 46 with
+    // one of 64).
     const bool few = t1 - t <= 2;
-    const bool narrow = a.window && a.window <= 16;
+    const bool narrow = a.window && a.window <= TILE;
     auto dots = [&](int t, const char* kt, const char* vt)
         __attribute__((always_inline)) {
       const int kv0 = t * TILE;

@@ -189,7 +189,7 @@ def test_attention_many_small_probabilities(T, dtype):
 
 @pytest.mark.parametrize("dtype", [FH, BF])
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("window", [2, 4, 8, 16])
+@pytest.mark.parametrize("window", [2, 4, 8, 16, 32, 64])
 def test_attention_narrow_window(window, D, dtype):
     """Rows of few keys: D owes nothing to a rounded o.  The mean error is a
     bound by itself (a value's rounding is off by 0.7 of u / sqrt(3) on the
